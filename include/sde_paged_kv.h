@@ -365,6 +365,91 @@ int sde_attention_dispatch(int attn_type, sde_kv_cache* cache, int layer,
                            void* d_workspace, size_t workspace_bytes,
                            sde_stream_t stream);
 
+/* ---- several requests over one pool --------------------------------------
+ * The reference decodes one sequence; a server that holds many keeps their
+ * blocks in one pool of the same layout and steps them together.  The calls
+ * below have no counterpart in the reference beyond the one-sequence kernels
+ * that each names.  They take the pool and every request's block table by
+ * pointer, and each request's length or position from device memory, so a
+ * captured graph replays with other lengths.  The current device must be the
+ * buffers' own.  Nothing on the host looks at device values: a position or
+ * table entry outside its range is left out by the kernels, as said at each.
+ * Calls write only what they name and keep nothing between calls; calls on
+ * different streams may overlap if they share no output and no workspace. */
+
+/* Element types of rows in and out. */
+enum { SDE_F32 = 0, SDE_F16 = 1, SDE_BF16 = 2 };
+
+/* A pool (sde_kv_view's layout: fp16 [pool_blocks][K, V][block_size][kv_dim])
+ * and one layer's block tables: position p of request s is in block
+ * tables[s * table_stride + p / block_size], slot p % block_size.
+ * block_size up to 1024; pool_blocks * 2 * block_size below 2^32 and
+ * max_blocks * block_size below 2^31 (SDE_ERR_UNSUPPORTED).  n_seqs == 0 makes
+ * every call a no-op. */
+typedef struct sde_batch_pool {
+  uint16_t* pool;
+  const int32_t* tables; /* device, [n_seqs][table_stride] */
+  int32_t pool_blocks;
+  int32_t block_size;
+  int32_t kv_dim;
+  int32_t n_seqs;
+  int32_t max_blocks;   /* entries of a request's table              */
+  int32_t table_stride; /* elements from one request's to the next's */
+} sde_batch_pool;
+
+/* RoPE + append of n_tokens tokens of several requests in one launch
+ * (cublas_rope_kernel kernels.cu:797-817 and cublas_kv_append_kernel
+ * kernels.cu:826-844): token t belongs to request d_seq[t] at position
+ * d_pos[t].  d_k and d_v are rows of nkv*dph elements of `dtype`, k_stride and
+ * v_stride elements apart (slices of a fused projection need no copy); k is
+ * rotated and both go to the pool as fp16 (round-to-nearest-even).  With d_q,
+ * rows of nh*dph elements are rotated into d_q_out, and with d_k_out the
+ * rotated k is written there too, both as `dtype`; an output may be its input
+ * (same pointer and stride), otherwise buffers must not overlap.  rope NULL
+ * rotates nothing.  The rotation is rotate-half, pairs (j, j+dph/2), by
+ * pos / div * theta^(-2j/dph) radians, scaling as in
+ * sde_rope_append_attention; here the angle is exact to 2^-32 turns at every
+ * position (frequencies in 64-bit fixed point), where the one-sequence call
+ * rounds frequency and angle to fp32, so at far positions the two rotate a
+ * little differently (position 30000: up to 2e-3 rad): a sequence keeps to
+ * one of them.
+ * Tokens whose request is outside [0, n_seqs) (padding), whose position is
+ * negative or beyond the table, or whose block is outside the pool are left
+ * out: nothing of theirs is written, q included.  Two tokens of one call at
+ * the same place: either is kept.  dph even, up to 512; kv_dim up to 2^20,
+ * n_tokens up to 2^23 (SDE_ERR_UNSUPPORTED). */
+int sde_batch_append(const sde_batch_pool* pool, const int32_t* d_seq, const int32_t* d_pos,
+                     int n_tokens, int dtype, const void* d_k, int64_t k_stride, const void* d_v,
+                     int64_t v_stride, void* d_k_out, int64_t k_out_stride, const void* d_q,
+                     int64_t q_stride, void* d_q_out, int64_t q_out_stride, int nh, int nkv,
+                     int dph, const sde_rope_config* rope, sde_stream_t stream);
+
+/* Workspace bytes of sde_batch_attention for these arguments (0 where the call
+ * needs none, or for shapes it does not take).  It needs no initialisation. */
+size_t sde_batch_attention_workspace_size(int n_seqs, int nh, int nkv, int dph, int n_queries,
+                                          int max_len, int block_size);
+
+/* Causal paged GQA attention of the newest n_queries tokens of each request
+ * (cublas_attention_kernel, kernels.cu:904-940, for a batch): request s has
+ * d_lens[s] positions, its new tokens' included (append first), and query i of
+ * it, row s*n_queries + i of d_q and d_out, sees positions
+ * [0, d_lens[s] - n_queries + i].  A query that sees nothing gives zeros.
+ * Lengths below 0 count as 0, above max_len as max_len; max_len, the bound
+ * that the launch is planned for, is at most max_blocks * block_size
+ * (SDE_ERR_CAPACITY).  Positions in blocks outside the pool are left out.
+ * Rows are nh*dph elements of `dtype`, q_stride and out_stride elements apart;
+ * logits, softmax and sums are fp32 (fp16 MFMA products of hi + lo parts: any
+ * finite q), the output is rounded once.  Nothing at positions that a query
+ * does not see reaches its output, NaN and infinities included; a V element
+ * that is not finite makes that output element not finite where it is seen.
+ * dph a multiple of 8 up to 256, n_queries up to 64, the pool 16-byte aligned
+ * (SDE_ERR_UNSUPPORTED).  d_workspace: 16-byte aligned,
+ * sde_batch_attention_workspace_size(...) bytes (SDE_ERR_WORKSPACE). */
+int sde_batch_attention(const sde_batch_pool* pool, const int32_t* d_lens, int n_queries,
+                        int max_len, int dtype, const void* d_q, int64_t q_stride, void* d_out,
+                        int64_t out_stride, int nh, int nkv, int dph, void* d_workspace,
+                        size_t workspace_bytes, sde_stream_t stream);
+
 /* Workspace bytes of sde_matvec and of the grid-cooperative device function
  * sde::device_matvec_grid (include/sde/matvec_device.hpp) for any call with
  * these shapes; 0 for invalid shapes.  Zero it once after allocation: its

@@ -59,6 +59,25 @@ class RopeConfig(ctypes.Structure):
     ]
 
 
+SDE_F32 = 0
+SDE_F16 = 1
+SDE_BF16 = 2
+
+
+class BatchPool(ctypes.Structure):
+    """sde_batch_pool: a pool and the block tables of several requests."""
+    _fields_ = [
+        ("pool", ctypes.c_void_p),
+        ("tables", ctypes.c_void_p),
+        ("pool_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("kv_dim", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("table_stride", ctypes.c_int32),
+    ]
+
+
 class KVView(ctypes.Structure):
     _fields_ = [
         ("pool", ctypes.c_void_p),
@@ -151,6 +170,7 @@ class LoopConfig(ctypes.Structure):
 _c_int = ctypes.c_int
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
+_i64 = ctypes.c_int64
 _cfg_p = ctypes.POINTER(KVConfig)
 _i32_p = ctypes.POINTER(ctypes.c_int32)
 
@@ -190,6 +210,11 @@ PROTOTYPES = {
                                            _c_int, _c_int, _c_int, _vp, _vp, _sz, _vp]),
     "sde_attention_dispatch": (_c_int, [_c_int, _vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int,
                                         _c_int, _c_int, _vp, _sz, _vp]),
+    "sde_batch_append": (_c_int, [_vp, _vp, _vp, _c_int, _c_int, _vp, _i64, _vp, _i64, _vp, _i64,
+                                  _vp, _i64, _vp, _i64, _c_int, _c_int, _c_int, _vp, _vp]),
+    "sde_batch_attention_workspace_size": (_sz, [_c_int] * 7),
+    "sde_batch_attention": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp, _i64, _vp, _i64,
+                                     _c_int, _c_int, _c_int, _vp, _sz, _vp]),
     "sde_matvec_workspace_size": (_sz, [_c_int, _c_int, _c_int]),
     "sde_model_read_header": (_c_int, [ctypes.c_char_p, ctypes.POINTER(ModelConfig)]),
     "sde_model_weights_bytes": (_sz, [ctypes.POINTER(ModelConfig)]),

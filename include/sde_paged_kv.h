@@ -450,6 +450,31 @@ int sde_batch_attention(const sde_batch_pool* pool, const int32_t* d_lens, int n
                         int64_t out_stride, int nh, int nkv, int dph, void* d_workspace,
                         size_t workspace_bytes, sde_stream_t stream);
 
+/* One token per row of logits, drawn under temperature, top-k, top-p and min-p
+ * from a given random number (the reference samples by temperature alone,
+ * softmax_sample_temperature_kernel, kernels.cu:285-317).  Row r is `vocab`
+ * elements of `dtype`, row_stride elements from the last; with
+ * w_i = exp((x_i - max x) / d_temperature[r]) and the tokens in order of falling
+ * x, ties by rising index:
+ *   the first d_top_k[r] of them (<= 0 or >= vocab: all);
+ *   of those the shortest run whose weight reaches d_top_p[r] of theirs
+ *     (>= 1: all; one token at least);
+ *   of those the ones with w >= d_min_p[r] (<= 0: all; above 1 acts as 1);
+ * and d_tokens[r] is the first index i whose kept weight, summed in index order
+ * up to and with i, is more than d_u[r] times the whole (u outside [0, 1): the
+ * first or last kept token).  d_probs[r], if d_probs is given, is that token's
+ * share of the kept weight.  A temperature below 1e-6 (or NaN) takes the
+ * largest logit, the first of equal ones.  Logits of -inf (and NaN, which
+ * counts as it) are never drawn; a row of nothing else gives token -1 and
+ * probability 0.  Logits of +inf share the row evenly.  Weights and sums are
+ * 64-bit.  The parameter arrays, one value per row on the device, may each be
+ * NULL: temperature 1, no filter.  vocab up to 2^24, n_rows up to 2^21
+ * (SDE_ERR_UNSUPPORTED). */
+int sde_sample(const void* d_logits, int64_t row_stride, int dtype, int n_rows, int vocab,
+               const float* d_u, const float* d_temperature, const int32_t* d_top_k,
+               const float* d_top_p, const float* d_min_p, int32_t* d_tokens, float* d_probs,
+               sde_stream_t stream);
+
 /* Workspace bytes of sde_matvec and of the grid-cooperative device function
  * sde::device_matvec_grid (include/sde/matvec_device.hpp) for any call with
  * these shapes; 0 for invalid shapes.  Zero it once after allocation: its

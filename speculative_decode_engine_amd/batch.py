@@ -1,5 +1,5 @@
 """Steps over several requests that share one paged pool: a ctypes mirror of
-sde_batch_append and sde_batch_attention (include/sde_paged_kv.h).
+sde_batch_append, sde_batch_attention and sde_sample (include/sde_paged_kv.h).
 
 The pool has KVCache's layout, float16 (or its int16 bits)
 [blocks][2][block_size][kv_dim]; `KVCache.pool_blocks_view()` is one.  A step of
@@ -7,6 +7,10 @@ a batch is, per layer,
 
     batch_append(pool, tables, seq, pos, k, v, nh, nkv, dph, q=q, q_out=q)
     out = batch_attention(q, pool, tables, lens, nh, nkv, dph)
+
+and at its end, over the rows of logits,
+
+    tokens, probs = sample(logits, u, temperature, top_k, top_p, min_p)
 
 with `tables` the layer's block tables, one row per request, and positions and
 lengths on the device: a captured graph replays with new ones.
@@ -172,3 +176,49 @@ def batch_attention(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor,
             ctypes.byref(d), lens.data_ptr(), n_queries, max_len, dtype, q.data_ptr(), qs,
             out.data_ptr(), os, nh, nkv, dph, ptr, size, _stream(stream)), "batch_attention")
     return out
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
+           top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+           min_p: Optional[torch.Tensor] = None, tokens: Optional[torch.Tensor] = None,
+           probs: Optional[torch.Tensor] = None,
+           stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """One token per row of logits [rows][vocab] (float32, float16 or bfloat16),
+    drawn with the random numbers u (float32 [rows], in [0, 1)): weights
+    exp(x / temperature), the top_k largest, of those the shortest run that
+    reaches top_p of their weight, of those the ones of at least min_p times the
+    largest; the token where the kept weight, summed by index, passes u of it.
+    Parameters are float32 (top_k int32) tensors of one value per row, or None
+    (temperature 1, no filter); a temperature below 1e-6 takes the largest
+    logit.  Returns tokens int32 [rows] (-1 where every logit is -inf or NaN)
+    and each one's probability among those kept."""
+    if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda" or logits.dim() != 2:
+        raise TypeError("logits must be a 2-D CUDA tensor")
+    dtype = _DTYPES.get(logits.dtype)
+    if dtype is None:
+        raise TypeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
+    dev, (n, V) = logits.device, logits.shape
+    stride = _rows(logits, "logits", n, V, logits.dtype, dev)
+    for t, name, want in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
+                          (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                          (min_p, "min_p", torch.float32), (tokens, "tokens", torch.int32),
+                          (probs, "probs", torch.float32)):
+        if t is None and name != "u":
+            continue
+        if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != want:
+            raise TypeError(f"{name} must be a {want} tensor on {dev}")
+        if t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous with shape {(n,)}, got {tuple(t.shape)}")
+    with _On(dev):
+        if tokens is None:
+            tokens = torch.empty(n, dtype=torch.int32, device=dev)
+        if probs is None:
+            probs = torch.empty(n, dtype=torch.float32, device=dev)
+        check(_native.load().sde_sample(
+            logits.data_ptr(), stride, dtype, n, V, u.data_ptr(),
+            None if temperature is None else temperature.data_ptr(),
+            None if top_k is None else top_k.data_ptr(),
+            None if top_p is None else top_p.data_ptr(),
+            None if min_p is None else min_p.data_ptr(), tokens.data_ptr(), probs.data_ptr(),
+            _stream(stream)), "sample")
+    return tokens, probs

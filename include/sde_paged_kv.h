@@ -450,6 +450,26 @@ int sde_batch_attention(const sde_batch_pool* pool, const int32_t* d_lens, int n
                         int64_t out_stride, int nh, int nkv, int dph, void* d_workspace,
                         size_t workspace_bytes, sde_stream_t stream);
 
+/* Causal attention of packed prompts within themselves (whole prompts, ahead of
+ * or beside their append): sequence b's tokens are rows d_starts[b] ..
+ * d_starts[b+1]-1 (device, n_seqs + 1 rising entries) of q and out, rows of
+ * nh*dph elements, and of k and v, rows of nkv*dph, all rotated already; query i
+ * of a sequence sees its keys 0 .. i, q head h KV head h*nkv/nh, scale
+ * dph^-1/2.  Where the reference prefills by cublas_attention_kernel, one
+ * sequence through the cache (kernels.cu:904-940).  Rows are `dtype`, SDE_F16 or
+ * SDE_BF16 (fp32 rows take sde_paged_attention), *_stride elements apart;
+ * logits, softmax and sums are fp32, a weight is rounded to `dtype` for its
+ * product with V.  n_tokens is the rows of the buffers: rows outside
+ * [d_starts[0], d_starts[n_seqs]) are left as they were, starts beyond it count
+ * as n_tokens, and starts that fall leave rows out.  Nothing of keys that a query
+ * does not see reaches its output, NaN and infinities included.  dph a multiple
+ * of 8 up to 256; buffers and strides multiples of 16 bytes
+ * (SDE_ERR_UNSUPPORTED).  No workspace. */
+int sde_prompt_attention(const int32_t* d_starts, int n_seqs, int n_tokens, int dtype,
+                         const void* d_q, int64_t q_stride, const void* d_k, int64_t k_stride,
+                         const void* d_v, int64_t v_stride, void* d_out, int64_t out_stride,
+                         int nh, int nkv, int dph, sde_stream_t stream);
+
 /* One token per row of logits, drawn under temperature, top-k, top-p and min-p
  * from a given random number (the reference samples by temperature alone,
  * softmax_sample_temperature_kernel, kernels.cu:285-317).  Row r is `vocab`

@@ -8,7 +8,8 @@ from .kv_cache import (ATTN_KDA, ATTN_LINEAR, ATTN_SLIDING_WINDOW, ATTN_SOFTMAX,
                        kv_cache_alloc, kv_cache_free, kv_cache_reset, spec_accept_greedy,
                        spec_accept_stochastic)
 from ._native import SDEError
-from .batch import batch_append, batch_attention, batch_attention_workspace_size, sample
+from .batch import (batch_append, batch_attention, batch_attention_workspace_size,
+                    prompt_attention, sample)
 from .matvec import PackedWeight, matvec, matvec_packed, matvec_workspace
 from .sdec import SDECModel, load_sdec, read_header, write_sdec
 from .spec_loop import SpecLoopModel, spec_loop_greedy, spec_loop_stochastic
@@ -17,5 +18,6 @@ __all__ = ["KVCache", "kv_cache_alloc", "kv_cache_free", "kv_cache_reset", "SDEE
            "spec_accept_greedy", "spec_accept_stochastic", "matvec", "matvec_workspace", "PackedWeight", "matvec_packed",
            "SDECModel", "load_sdec", "read_header", "write_sdec",
            "SpecLoopModel", "spec_loop_greedy", "spec_loop_stochastic",
-           "batch_append", "batch_attention", "batch_attention_workspace_size", "sample",
+           "batch_append", "batch_attention", "batch_attention_workspace_size",
+           "prompt_attention", "sample",
            "ATTN_SOFTMAX", "ATTN_SLIDING_WINDOW", "ATTN_KDA", "ATTN_LINEAR"]

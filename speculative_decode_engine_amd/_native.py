@@ -215,6 +215,8 @@ PROTOTYPES = {
     "sde_batch_attention_workspace_size": (_sz, [_c_int] * 7),
     "sde_batch_attention": (_c_int, [_vp, _vp, _c_int, _c_int, _c_int, _vp, _i64, _vp, _i64,
                                      _c_int, _c_int, _c_int, _vp, _sz, _vp]),
+    "sde_prompt_attention": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _i64, _vp, _i64, _vp, _i64,
+                                      _vp, _i64, _c_int, _c_int, _c_int, _vp]),
     "sde_sample": (_c_int, [_vp, _i64, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                             _vp]),
     "sde_matvec_workspace_size": (_sz, [_c_int, _c_int, _c_int]),

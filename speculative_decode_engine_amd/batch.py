@@ -1,5 +1,6 @@
 """Steps over several requests that share one paged pool: a ctypes mirror of
-sde_batch_append, sde_batch_attention and sde_sample (include/sde_paged_kv.h).
+sde_batch_append, sde_batch_attention, sde_prompt_attention and sde_sample
+(include/sde_paged_kv.h).
 
 The pool has KVCache's layout, float16 (or its int16 bits)
 [blocks][2][block_size][kv_dim]; `KVCache.pool_blocks_view()` is one.  A step of
@@ -8,7 +9,8 @@ a batch is, per layer,
     batch_append(pool, tables, seq, pos, k, v, nh, nkv, dph, q=q, q_out=q)
     out = batch_attention(q, pool, tables, lens, nh, nkv, dph)
 
-and at its end, over the rows of logits,
+(new prompts, packed, take `prompt_attention` over the rotated rows) and at its
+end, over the rows of logits,
 
     tokens, probs = sample(logits, u, temperature, top_k, top_p, min_p)
 
@@ -175,6 +177,38 @@ def batch_attention(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor,
         check(lib.sde_batch_attention(
             ctypes.byref(d), lens.data_ptr(), n_queries, max_len, dtype, q.data_ptr(), qs,
             out.data_ptr(), os, nh, nkv, dph, ptr, size, _stream(stream)), "batch_attention")
+    return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor,
+                     nh: int, nkv: int, dph: int, out: Optional[torch.Tensor] = None,
+                     stream=None) -> torch.Tensor:
+    """Causal attention of packed prompts within themselves: sequence b's tokens
+    are rows starts[b] .. starts[b+1]-1 (int32, on the device) of q and out
+    [T][nh*dph] and of k and v [T][nkv*dph], float16 or bfloat16, rotated
+    already.  Rows may be slices of a fused projection (multiples of 16 bytes).
+    Rows outside the sequences are left as they were (zeros where out is
+    allocated here)."""
+    if not isinstance(q, torch.Tensor) or q.device.type != "cuda" or q.dim() != 2:
+        raise TypeError("q must be a 2-D CUDA tensor")
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None or dtype == _native.SDE_F32:
+        raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
+    dev, T = q.device, q.shape[0]
+    qs = _rows(q, "q", T, nh * dph, q.dtype, dev)
+    ks = _rows(k, "k", T, nkv * dph, q.dtype, dev)
+    vs = _rows(v, "v", T, nkv * dph, q.dtype, dev)
+    if not isinstance(starts, torch.Tensor) or starts.dim() != 1 or starts.shape[0] < 1:
+        raise ValueError("starts must have one entry per sequence and one for the end")
+    _ints(starts, "starts", starts.shape[0], dev)
+    with _On(dev):
+        if out is None:
+            out = torch.zeros(T, nh * dph, dtype=q.dtype, device=dev)
+        os = _rows(out, "out", T, nh * dph, q.dtype, dev)
+        check(_native.load().sde_prompt_attention(
+            starts.data_ptr(), starts.shape[0] - 1, T, dtype, q.data_ptr(), qs, k.data_ptr(), ks,
+            v.data_ptr(), vs, out.data_ptr(), os, nh, nkv, dph, _stream(stream)),
+            "prompt_attention")
     return out
 
 

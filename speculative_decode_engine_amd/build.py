@@ -24,7 +24,7 @@ OFFLOAD_ARCH = "gfx950"
 
 SOURCES = ["kv_cache.hip", "paged_attention.hip", "attention_window.hip",
            "attention_generic.hip", "spec_accept.hip", "matvec.hip", "model_loader.hip", "spec_loop.hip",
-           "batch_append.hip", "batch_attention.hip", "sample.hip"]
+           "batch_append.hip", "batch_attention.hip", "prompt_attention.hip", "sample.hip"]
 
 # Measurement kernels for bench.py (a streaming read and the attention's
 # load skeleton): a library of their own, not part of the product.

@@ -470,6 +470,10 @@ int sde_prompt_attention(const int32_t* d_starts, int n_seqs, int n_tokens, int 
                          const void* d_v, int64_t v_stride, void* d_out, int64_t out_stride,
                          int nh, int nkv, int dph, sde_stream_t stream);
 
+/* Workspace bytes of sde_sample (0 where it needs none).  It needs no
+ * initialisation. */
+size_t sde_sample_workspace_size(int n_rows, int vocab);
+
 /* One token per row of logits, drawn under temperature, top-k, top-p and min-p
  * from a given random number (the reference samples by temperature alone,
  * softmax_sample_temperature_kernel, kernels.cu:285-317).  Row r is `vocab`
@@ -489,11 +493,12 @@ int sde_prompt_attention(const int32_t* d_starts, int n_seqs, int n_tokens, int 
  * probability 0.  Logits of +inf share the row evenly.  Weights and sums are
  * 64-bit.  The parameter arrays, one value per row on the device, may each be
  * NULL: temperature 1, no filter.  vocab up to 2^24, n_rows up to 2^21
- * (SDE_ERR_UNSUPPORTED). */
+ * (SDE_ERR_UNSUPPORTED).  d_workspace: 16-byte aligned,
+ * sde_sample_workspace_size(...) bytes (SDE_ERR_WORKSPACE). */
 int sde_sample(const void* d_logits, int64_t row_stride, int dtype, int n_rows, int vocab,
                const float* d_u, const float* d_temperature, const int32_t* d_top_k,
                const float* d_top_p, const float* d_min_p, int32_t* d_tokens, float* d_probs,
-               sde_stream_t stream);
+               void* d_workspace, size_t workspace_bytes, sde_stream_t stream);
 
 /* Workspace bytes of sde_matvec and of the grid-cooperative device function
  * sde::device_matvec_grid (include/sde/matvec_device.hpp) for any call with

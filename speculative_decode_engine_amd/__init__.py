@@ -9,7 +9,7 @@ from .kv_cache import (ATTN_KDA, ATTN_LINEAR, ATTN_SLIDING_WINDOW, ATTN_SOFTMAX,
                        spec_accept_stochastic)
 from ._native import SDEError
 from .batch import (batch_append, batch_attention, batch_attention_workspace_size,
-                    prompt_attention, sample)
+                    prompt_attention, sample, sample_workspace_size)
 from .matvec import PackedWeight, matvec, matvec_packed, matvec_workspace
 from .sdec import SDECModel, load_sdec, read_header, write_sdec
 from .spec_loop import SpecLoopModel, spec_loop_greedy, spec_loop_stochastic
@@ -19,5 +19,5 @@ __all__ = ["KVCache", "kv_cache_alloc", "kv_cache_free", "kv_cache_reset", "SDEE
            "SDECModel", "load_sdec", "read_header", "write_sdec",
            "SpecLoopModel", "spec_loop_greedy", "spec_loop_stochastic",
            "batch_append", "batch_attention", "batch_attention_workspace_size",
-           "prompt_attention", "sample",
+           "prompt_attention", "sample", "sample_workspace_size",
            "ATTN_SOFTMAX", "ATTN_SLIDING_WINDOW", "ATTN_KDA", "ATTN_LINEAR"]

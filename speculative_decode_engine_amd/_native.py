@@ -217,8 +217,9 @@ PROTOTYPES = {
                                      _c_int, _c_int, _c_int, _vp, _sz, _vp]),
     "sde_prompt_attention": (_c_int, [_vp, _c_int, _c_int, _c_int, _vp, _i64, _vp, _i64, _vp, _i64,
                                       _vp, _i64, _c_int, _c_int, _c_int, _vp]),
+    "sde_sample_workspace_size": (_sz, [_c_int, _c_int]),
     "sde_sample": (_c_int, [_vp, _i64, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-                            _vp]),
+                            _vp, _sz, _vp]),
     "sde_matvec_workspace_size": (_sz, [_c_int, _c_int, _c_int]),
     "sde_model_read_header": (_c_int, [ctypes.c_char_p, ctypes.POINTER(ModelConfig)]),
     "sde_model_weights_bytes": (_sz, [ctypes.POINTER(ModelConfig)]),

@@ -88,6 +88,20 @@ def _pool(pool, tables, kv_dim: int) -> BatchPool:
                      blocks, tables.stride(0) if n > 1 else blocks)
 
 
+def _workspace(given: Optional[torch.Tensor], need: int, device, stream):
+    """(pointer, bytes, tensor) of the caller's workspace or of a new one."""
+    if given is None:
+        if need == 0:
+            return None, 0, None
+        given = torch.empty(need, dtype=torch.uint8, device=device)
+        if stream is not None:
+            given.record_stream(stream)
+        return given.data_ptr(), need, given
+    if given.device != device or not given.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+    return given.data_ptr(), given.numel() * given.element_size(), given
+
+
 def batch_append(pool: torch.Tensor, tables: torch.Tensor, seq: torch.Tensor, pos: torch.Tensor,
                  k: torch.Tensor, v: torch.Tensor, nh: int, nkv: int, dph: int,
                  theta: float = 10000.0, scaling_type: int = 0, scaling_factor: float = 1.0,
@@ -162,18 +176,9 @@ def batch_attention(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor,
             out = torch.empty(n * n_queries, nh * dph, dtype=q.dtype, device=dev)
         os = _rows(out, "out", n * n_queries, nh * dph, q.dtype, dev)
         lib = _native.load()
-        ptr, size = None, 0
-        if workspace is None:
-            size = lib.sde_batch_attention_workspace_size(n, nh, nkv, dph, n_queries, max_len,
-                                                          d.block_size)
-            if size:
-                workspace = torch.empty(size, dtype=torch.uint8, device=dev)
-                if stream is not None:
-                    workspace.record_stream(stream)
-        elif workspace.device != dev or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be a contiguous tensor on {dev}")
-        if workspace is not None:
-            ptr, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        ptr, size, workspace = _workspace(
+            workspace, lib.sde_batch_attention_workspace_size(n, nh, nkv, dph, n_queries, max_len,
+                                                              d.block_size), dev, stream)
         check(lib.sde_batch_attention(
             ctypes.byref(d), lens.data_ptr(), n_queries, max_len, dtype, q.data_ptr(), qs,
             out.data_ptr(), os, nh, nkv, dph, ptr, size, _stream(stream)), "batch_attention")
@@ -212,10 +217,14 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     return out
 
 
+def sample_workspace_size(n_rows: int, vocab: int) -> int:
+    return int(_native.load().sde_sample_workspace_size(n_rows, vocab))
+
+
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Tensor] = None,
            top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
            min_p: Optional[torch.Tensor] = None, tokens: Optional[torch.Tensor] = None,
-           probs: Optional[torch.Tensor] = None,
+           probs: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
            stream=None) -> tuple[torch.Tensor, torch.Tensor]:
     """One token per row of logits [rows][vocab] (float32, float16 or bfloat16),
     drawn with the random numbers u (float32 [rows], in [0, 1)): weights
@@ -225,7 +234,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     Parameters are float32 (top_k int32) tensors of one value per row, or None
     (temperature 1, no filter); a temperature below 1e-6 takes the largest
     logit.  Returns tokens int32 [rows] (-1 where every logit is -inf or NaN)
-    and each one's probability among those kept."""
+    and each one's probability among those kept.  The workspace
+    (sample_workspace_size bytes) is taken from torch's allocator when None."""
     if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda" or logits.dim() != 2:
         raise TypeError("logits must be a 2-D CUDA tensor")
     dtype = _DTYPES.get(logits.dtype)
@@ -248,11 +258,14 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
             tokens = torch.empty(n, dtype=torch.int32, device=dev)
         if probs is None:
             probs = torch.empty(n, dtype=torch.float32, device=dev)
-        check(_native.load().sde_sample(
+        lib = _native.load()
+        ptr, size, workspace = _workspace(workspace, lib.sde_sample_workspace_size(n, V), dev,
+                                          stream)
+        check(lib.sde_sample(
             logits.data_ptr(), stride, dtype, n, V, u.data_ptr(),
             None if temperature is None else temperature.data_ptr(),
             None if top_k is None else top_k.data_ptr(),
             None if top_p is None else top_p.data_ptr(),
             None if min_p is None else min_p.data_ptr(), tokens.data_ptr(), probs.data_ptr(),
-            _stream(stream)), "sample")
+            ptr, size, _stream(stream)), "sample")
     return tokens, probs

@@ -41,11 +41,15 @@ using batch::bf16_elem;
 using batch::f16_elem;
 using batch::f32_elem;
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;        // of a row's workgroup
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2048;           // histogram bins, 1/32 of a factor 2 each
+constexpr int kBins = 2048;           // its histogram bins, 1/32 of a factor 2 each
 constexpr float kBinsPerLog2 = 32.f;  // so tokens below 2^-64 of the largest are left out
 constexpr int kList = 512;            // tokens compared in LDS
+constexpr int kSliceThreads = 256;    // of a slice's workgroup
+constexpr int kSliceWaves = kSliceThreads / 64;
+constexpr int kSliceBins = 1024;
+constexpr int kMaxSlices = 64;
 constexpr float kMinTemperature = 1e-6f;
 constexpr int kMaxVocab = 1 << 24;
 
@@ -66,6 +70,10 @@ struct SampleArgs {
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+__device__ __forceinline__ float value_of_key(uint32_t k) {
+  return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
 // 2^t for t <= 0, to 1e-14 of it: the integer part to the exponent, the rest
@@ -94,16 +102,17 @@ struct Weight {
   float top;      // the row's max
   double per;     // log2(e) / T
   float bins;     // histogram bins per unit of (max - x) / 2
+  int limit;      // and their number
   __device__ __forceinline__ double of(float x) const {
     if (x == top) return 1.0;
     if (x == -INFINITY) return 0.0;
     return exp2_f64(((double)x - (double)top) * per);
   }
-  // 0 at the max, rising as x falls; kBins: left out
+  // 0 at the max, rising as x falls; `limit`: left out
   __device__ __forceinline__ int bin(float x) const {
     if (x == top) return 0;
-    if (x == -INFINITY) return kBins;
-    return (int)fminf((0.5f * top - 0.5f * x) * bins, (float)kBins);  // (halves: no overflow)
+    if (x == -INFINITY) return limit;
+    return (int)fminf((0.5f * top - 0.5f * x) * bins, (float)limit);  // (halves: no overflow)
   }
 };
 
@@ -194,11 +203,14 @@ struct Lds {
   double out_d[2];
   int out_i[2];
   uint32_t out_u[2];
+  uint32_t upto[64];
+  double slice_w[kMaxSlices];
 };
 
 __device__ __forceinline__ double shfl_up_d(double x, int d) { return __shfl_up(x, d, 64); }
 
 // Inclusive sum over the workgroup in thread order; `total` to every thread.
+template <int W = kWaves>
 __device__ __forceinline__ double block_scan(double x, double* wave_tot, double& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -211,7 +223,7 @@ __device__ __forceinline__ double block_scan(double x, double* wave_tot, double&
   __syncthreads();
   double before = 0.0, all = 0.0;
 #pragma unroll
-  for (int w = 0; w < kWaves; w++) {
+  for (int w = 0; w < W; w++) {
     const double t = wave_tot[w];
     if (w < wave) before += t;
     all += t;
@@ -220,6 +232,7 @@ __device__ __forceinline__ double block_scan(double x, double* wave_tot, double&
   return before + x;
 }
 
+template <int W = kWaves>
 __device__ __forceinline__ uint32_t block_scan_u(uint32_t x, uint32_t* wave_tot) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -232,7 +245,7 @@ __device__ __forceinline__ uint32_t block_scan_u(uint32_t x, uint32_t* wave_tot)
   __syncthreads();
   uint32_t before = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; w++)
+  for (int w = 0; w < W; w++)
     if (w < wave) before += wave_tot[w];
   return before + x;
 }
@@ -305,50 +318,19 @@ __device__ __forceinline__ BinAt find_bin(Lds& s, uint32_t k, double m, double u
   return at;
 }
 
-// The first index where the running sum of f(value, index) >= 0 in index order
-// passes `share` of the total (SHARE) or `share` itself, by a walk of the row
-// and one of the 16th that holds it.  Every thread gets the index (-1: the sum
-// is zero), its f and the total.
 struct Found {
   int index;
   double f, total;
 };
 
-template <bool SHARE, class E, class F>
-__device__ __forceinline__ Found find_index(const RowView<E>& row, double share, Lds& s, F f) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int per = (row.vectors + kWaves - 1) / kWaves;
-  double x = 0.0;
-  row.walk(min(wave * per, row.vectors), min((wave + 1) * per, row.vectors),
-           [&](float v, int i) { x += f(v, i); });
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+// The first index within vectors [v0, v1) where `base` and the running sum of f
+// pass `target` (the last with f > 0 where rounding leaves none): the vectors
+// in order over all threads, then one thread's.
+template <class E, class F>
+__device__ __forceinline__ Found find_within(const RowView<E>& row, int v0, int v1, double base,
+                                             double target, Lds& s, F f) {
   __syncthreads();
-  if (lane == 0) s.wave_d2[wave] = x;
   if (threadIdx.x == 0) s.out_i[0] = -1;
-  __syncthreads();
-  Found r{-1, 0.0, 0.0};
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) r.total += s.wave_d2[w];
-  if (!(r.total > 0.0)) {
-    __syncthreads();
-    return r;
-  }
-  const double target = SHARE ? share * r.total : share;
-  int ws = -1;
-  double base = 0.0, run = 0.0;
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) {
-    const double t = s.wave_d2[w];
-    // (the last wave with weight takes what rounding leaves over)
-    if (t > 0.0 && (ws < 0 || !(base + s.wave_d2[ws] > target))) {
-      ws = w;
-      base = run;
-    }
-    run += t;
-  }
-  // the wave's vectors, in order, over all threads
-  const int v0 = ws * per, v1 = min(v0 + per, row.vectors);
   const int each = (v1 - v0 + kThreads - 1) / kThreads;
   const int a = min(v0 + (int)threadIdx.x * each, v1), b = min(a + each, v1);
   double mine = 0.0;
@@ -410,10 +392,64 @@ __device__ __forceinline__ Found find_index(const RowView<E>& row, double share,
     }
   }
   __syncthreads();
-  r.index = s.out_i[0];
-  r.f = s.out_d[0];
+  const Found r{s.out_i[0], s.out_d[0], 0.0};
   __syncthreads();
   return r;
+}
+
+// The first index where the running sum of f(value, index) >= 0 in index order
+// passes `share` of the total (SHARE) or `share` itself, by a walk of the row
+// and one of the 16th that holds it.  Every thread gets the index (-1: the sum
+// is zero), its f and the total.
+template <bool SHARE, class E, class F>
+__device__ __forceinline__ Found find_index(const RowView<E>& row, double share, Lds& s, F f) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int per = (row.vectors + kWaves - 1) / kWaves;
+  double x = 0.0;
+  row.walk(min(wave * per, row.vectors), min((wave + 1) * per, row.vectors),
+           [&](float v, int i) { x += f(v, i); });
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d, 64);
+  __syncthreads();
+  if (lane == 0) s.wave_d2[wave] = x;
+  __syncthreads();
+  Found r{-1, 0.0, 0.0};
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) r.total += s.wave_d2[w];
+  if (!(r.total > 0.0)) {
+    __syncthreads();
+    return r;
+  }
+  const double target = SHARE ? share * r.total : share;
+  int ws = -1;
+  double base = 0.0, run = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) {
+    const double t = s.wave_d2[w];
+    // (the last wave with weight takes what rounding leaves over)
+    if (t > 0.0 && (ws < 0 || !(base + s.wave_d2[ws] > target))) {
+      ws = w;
+      base = run;
+    }
+    run += t;
+  }
+  const int v0 = ws * per;
+  const Found in = find_within(row, v0, min(v0 + per, row.vectors), base, target, s, f);
+  r.index = in.index;
+  r.f = in.f;
+  return r;
+}
+
+// s.key2 / s.index2 to s.key / s.index in index order.
+__device__ __forceinline__ void sort_list(Lds& s, int n) {
+  if ((int)threadIdx.x < n) {
+    const int me = s.index2[threadIdx.x];
+    int at = 0;
+    for (int j = 0; j < n; j++) at += s.index2[j] < me ? 1 : 0;
+    s.key[at] = s.key2[threadIdx.x];
+    s.index[at] = me;
+  }
+  __syncthreads();
 }
 
 // Gathers the tokens for which `in` holds into s.key / s.index in index order;
@@ -437,19 +473,8 @@ __device__ __forceinline__ int gather(const RowView<E>& row, Lds& s, P in) {
   __syncthreads();
   const uint32_t n = s.n;
   if (n > kList) return kList + 1;
-  if (threadIdx.x < n) {
-    const int me = s.index2[threadIdx.x];
-    int at = 0;
-    for (uint32_t j = 0; j < n; j++) at += s.index2[j] < me ? 1 : 0;
-    s.key[at] = s.key2[threadIdx.x];
-    s.index[at] = me;
-  }
-  __syncthreads();
+  sort_list(s, (int)n);
   return (int)n;
-}
-
-__device__ __forceinline__ float value_of_key(uint32_t k) {
-  return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
 // Rank of listed token i among the n listed (falling value, rising index) and
@@ -572,86 +597,550 @@ __device__ __forceinline__ Kept last_kept(const RowView<E>& row, const Weight& w
   }
 }
 
+// ---- few rows: a row in slices ---------------------------------------------
+//
+// One workgroup walks a row of 128256 at some 20 us a time where weights are
+// needed.  With fewer rows than fill the chip, a row is cut into slices of
+// vectors, a workgroup each, in three launches before the row's own:
+//  max      the slice's max, and each thread's for top-k;
+//  weights  top-k: the cut, a bound of the k-th largest (one workgroup a row);
+//           top-p: the slice's total and histogram; the last workgroup of a row
+//           joins them and finds the bin that holds the last kept token;
+//           neither: the slice's total;
+//  gather   the tokens at or above the cut, or in that bin, into a list per
+//           slice, and the slice's weight before the bin.
+// The row's workgroup then has the lists to compare, and the slices' weights
+// to find the one that holds the token, which alone it walks.
+// Which way a row goes is told by its parameters; one whose list would be too
+// long (flat rows, ties, k above kList) is walked whole by its workgroup.
+
+enum class Way { kTop, kTopK, kNucleus, kTotals, kWhole };
+
+struct RowParams {
+  float T, p;
+  double u, min_p;
+  int k;
+  bool has_k, has_p;
+  Way way;
+  __device__ __forceinline__ RowParams(const SampleArgs& a, int r) {
+    T = a.temperature ? a.temperature[r] : 1.f;
+    u = a.u[r];
+    k = a.top_k ? a.top_k[r] : 0;
+    p = a.top_p ? a.top_p[r] : 1.f;
+    min_p = a.min_p && a.min_p[r] > 0.f ? fmin((double)a.min_p[r], 1.0) : 0.0;
+    has_k = k > 0 && k < a.V;
+    has_p = p < 1.f;
+    if (!(T >= kMinTemperature))
+      way = Way::kTop;
+    else if (has_k)
+      way = k <= kList ? Way::kTopK : Way::kWhole;
+    else
+      way = has_p ? Way::kNucleus : Way::kTotals;
+  }
+  // tokens of less weight are never the last of a nucleus (half of it: sums
+  // are rounded)
+  __device__ __forceinline__ double least(int V) const {
+    return 0.5 * (1.0 - fmax((double)p, 0.0)) / (double)V;
+  }
+};
+
+// Fixed point of the histograms' weights: V of them fit 63 bits.
+__device__ __forceinline__ double fixed_point(int V) { return ldexp(1.0, 30 + __clz(V)); }
+
+struct SliceInfo {  // of a row
+  float cut;        // top-k: the lowest value listed
+  int lo, hi;       // top-p: the bins listed (lo < 0: none could be told)
+  uint32_t before;  // tokens before them
+  double below;     // and their weight
+  double all;       // the row's
+};
+
+struct SliceArgs {
+  SampleArgs a;
+  int S;                      // slices of a row
+  float* top;                 // [rows][S]
+  int* first;                 // [rows][S]
+  float* thread_top;          // [rows][S][kSliceThreads]
+  double* total;              // [rows][S]; after the gather: the weight before bin lo
+  unsigned long long* mass;   // [rows][S][kSliceBins]
+  uint32_t* count;            // [rows][S][kSliceBins]
+  uint32_t* listed;           // [rows][S]
+  uint2* list;                // [rows][S][kList]: key, index
+  SliceInfo* info;            // [rows]
+  uint32_t* arrived;          // [rows]
+};
+
+struct SliceLds {
+  uint32_t count[kSliceBins];
+  unsigned long long mass[kSliceBins];
+  double wave_d[kSliceWaves];
+  uint32_t wave_u[kSliceWaves];
+  float wave_f[kSliceWaves];
+  int wave_i[kSliceWaves];
+  int bin;
+  uint32_t n, key;
+  bool last;
+};
+
 template <class E>
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
+struct SliceView {
+  RowView<E> row;
+  int v0, v1;  // the slice's vectors
+  int w0, w1;  // the wave's
+  __device__ __forceinline__ SliceView(const SliceArgs& sa, int r, int s)
+      : row(sa.a.logits, r * sa.a.row_stride, sa.a.V) {
+    const int per = (row.vectors + sa.S - 1) / sa.S;
+    v0 = min(s * per, row.vectors);
+    v1 = min(v0 + per, row.vectors);
+    const int wave = threadIdx.x >> 6;
+    const int wp = (v1 - v0 + kSliceWaves - 1) / kSliceWaves;
+    w0 = min(v0 + wave * wp, v1);
+    w1 = min(w0 + wp, v1);
+  }
+};
+
+// (max, first index of it) over the lanes.
+__device__ __forceinline__ void wave_top(float& x, int& i) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const float y = __shfl_xor(x, d, 64);
+    const int j = __shfl_xor(i, d, 64);
+    if (y > x || (y == x && (uint32_t)j < (uint32_t)i)) {
+      x = y;
+      i = j;
+    }
+  }
+}
+
+// The row's, from its slices'.
+__device__ __forceinline__ void row_top(const SliceArgs& sa, int r, float& x, int& i) {
+  const int lane = threadIdx.x & 63;
+  x = -INFINITY;
+  i = -1;
+  if (lane < sa.S) {
+    x = sa.top[r * sa.S + lane];
+    i = sa.first[r * sa.S + lane];
+  }
+  wave_top(x, i);
+}
+
+// The bins of a nucleus: from the max down to the least weight that can be its
+// last.
+__device__ __forceinline__ Weight nucleus_weight(const RowParams& q, float top, int V) {
+  Weight w;
+  w.top = top;
+  w.per = 1.4426950408889634 / (double)q.T;
+  const float range = log2f((float)V / (1.f - fmaxf(q.p, 0.f))) + 2.f;
+  w.bins = 2.f * (float)w.per * ((float)kSliceBins / range);
+  w.limit = kSliceBins;
+  return w;
+}
+
+template <class E>
+__global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SliceArgs sa) {
+  __shared__ SliceLds s;
+  const int r = blockIdx.y, sl = blockIdx.x, tid = threadIdx.x;
+  const SliceView<E> view(sa, r, sl);
+  float x = -INFINITY;
+  int i = -1;
+  view.row.walk(view.w0, view.w1, [&](float v, int at) {
+    if (v > x) {
+      x = v;
+      i = at;
+    }
+  });
+  const size_t rs = (size_t)r * sa.S + sl;
+  if (RowParams(sa.a, r).way == Way::kTopK) sa.thread_top[rs * kSliceThreads + tid] = x;
+  wave_top(x, i);
+  if ((tid & 63) == 0) {
+    s.wave_f[tid >> 6] = x;
+    s.wave_i[tid >> 6] = i;
+  }
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 1; w < kSliceWaves; w++)
+      if (s.wave_f[w] > x) {
+        x = s.wave_f[w];
+        i = s.wave_i[w];
+      }
+    sa.top[rs] = x;
+    sa.first[rs] = i;
+    if (sl == 0) sa.arrived[r] = 0;
+  }
+}
+
+// The lowest of the threads' maxima that at least k of them reach (to a bin's
+// width): at least k tokens do.
+__device__ __forceinline__ float top_k_cut(const SliceArgs& sa, int r, int k, float top,
+                                           SliceLds& s) {
+  const int tid = threadIdx.x, n = sa.S * kSliceThreads;
+  const float* t = sa.thread_top + (size_t)r * n;
+  for (int i = tid; i < kSliceBins; i += kSliceThreads) s.count[i] = 0;
+  if (tid == 0) {
+    s.key = 0xFFFFFFFFu;
+    s.bin = kSliceBins;
+    s.n = 0;
+  }
+  __syncthreads();
+  float low = INFINITY;
+  uint32_t live = 0;
+  for (int i = tid; i < n; i += kSliceThreads) {
+    const float x = t[i];
+    if (x > -INFINITY) {
+      low = fminf(low, x);
+      live++;
+    }
+  }
+  if (live > 0) {
+    atomicMin(&s.key, key_of(low));
+    atomicAdd(&s.n, live);
+  }
+  __syncthreads();
+  if (s.n < (uint32_t)k) return -FLT_MAX;  // every token with a weight
+  low = value_of_key(s.key);
+  const float span = 0.5f * top - 0.5f * low;
+  const float scale = span > 0.f && span < INFINITY ? (float)(kSliceBins - 1) / span : 0.f;
+  auto bin = [&](float x) {
+    return x == top ? 0 : (int)fminf((0.5f * top - 0.5f * x) * scale, (float)(kSliceBins - 1));
+  };
+  for (int i = tid; i < n; i += kSliceThreads) {
+    const float x = t[i];
+    if (x > -INFINITY) atomicAdd(&s.count[bin(x)], 1u);
+  }
+  __syncthreads();
+  constexpr int PER = kSliceBins / kSliceThreads;
+  uint32_t c = 0;
+  for (int i = 0; i < PER; i++) c += s.count[tid * PER + i];
+  uint32_t run = block_scan_u<kSliceWaves>(c, s.wave_u) - c;
+  for (int i = 0; i < PER; i++) {
+    run += s.count[tid * PER + i];
+    if (run >= (uint32_t)k) {
+      atomicMin(&s.bin, tid * PER + i);
+      break;
+    }
+  }
+  if (tid == 0) s.key = 0xFFFFFFFFu;
+  __syncthreads();
+  const int b = s.bin;
+  low = INFINITY;
+  for (int i = tid; i < n; i += kSliceThreads) {
+    const float x = t[i];
+    if (x > -INFINITY && bin(x) <= b) low = fminf(low, x);
+  }
+  if (low < INFINITY) atomicMin(&s.key, key_of(low));
+  __syncthreads();
+  return s.key == 0xFFFFFFFFu ? top : value_of_key(s.key);
+}
+
+template <class E>
+__global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs sa) {
+  __shared__ SliceLds s;
+  const int r = blockIdx.y, sl = blockIdx.x, tid = threadIdx.x;
+  const RowParams q(sa.a, r);
+  if (q.way == Way::kTop || q.way == Way::kWhole || (q.way == Way::kTopK && sl > 0)) return;
+  float top;
+  int first;
+  row_top(sa, r, top, first);
+  if (first < 0) return;
+  if (q.way == Way::kTopK) {
+    const float cut = top_k_cut(sa, r, q.k, top, s);
+    if (tid == 0) sa.info[r].cut = cut;
+    return;
+  }
+  const SliceView<E> view(sa, r, sl);
+  const size_t rs = (size_t)r * sa.S + sl;
+  const Weight weight = nucleus_weight(q, top, sa.a.V);
+  double x = 0.0, all;
+  if (q.way == Way::kTotals) {
+    view.row.walk(view.w0, view.w1, [&](float v, int) {
+      const double w = weight.of(v);
+      x += w >= q.min_p ? w : 0.0;
+    });
+    block_scan<kSliceWaves>(x, s.wave_d, all);
+    if (tid == 0) sa.total[rs] = all;
+    return;
+  }
+  const double fixed = fixed_point(sa.a.V), least = q.least(sa.a.V);
+  for (int i = tid; i < kSliceBins; i += kSliceThreads) {
+    s.count[i] = 0;
+    s.mass[i] = 0;
+  }
+  __syncthreads();
+  view.row.walk(view.w0, view.w1, [&](float v, int) {
+    const double w = weight.of(v);
+    x += w;
+    const int b = weight.bin(v);
+    if (w >= least && b < kSliceBins) {
+      atomicAdd(&s.count[b], 1u);
+      atomicAdd(&s.mass[b], (unsigned long long)(w * fixed + 0.5));
+    }
+  });
+  block_scan<kSliceWaves>(x, s.wave_d, all);
+  // Published by agent-scope stores, which write through; every wave waits for
+  // its own before the arrival is counted.
+  for (int i = tid; i < kSliceBins; i += kSliceThreads) {
+    __hip_atomic_store(sa.mass + rs * kSliceBins + i, s.mass[i], __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(sa.count + rs * kSliceBins + i, s.count[i], __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (tid == 0)
+    __hip_atomic_store(reinterpret_cast<unsigned long long*>(sa.total + rs),
+                       __builtin_bit_cast(unsigned long long, all), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+  __syncthreads();
+  if (tid == 0)
+    s.last = __hip_atomic_fetch_add(sa.arrived + r, 1u, __ATOMIC_RELAXED,
+                                    __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)sa.S - 1;
+  __syncthreads();
+  if (!s.last) return;
+
+  // ---- the row's histogram, and the bin of the last kept token
+  constexpr int PER = kSliceBins / kSliceThreads;
+  const size_t r0 = (size_t)r * sa.S;
+  unsigned long long m[PER] = {};
+  uint32_t c[PER] = {};
+#pragma unroll 4
+  for (int i = 0; i < sa.S; i++) {
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const size_t at = (r0 + i) * kSliceBins + tid * PER + j;
+      m[j] += __hip_atomic_load(sa.mass + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      c[j] += __hip_atomic_load(sa.count + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  all = 0.0;
+  for (int i = 0; i < sa.S; i++)
+    all += __builtin_bit_cast(
+        double, __hip_atomic_load(reinterpret_cast<unsigned long long*>(sa.total + r0 + i),
+                                  __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  const double unit = 1.0 / fixed, target = (double)q.p * all;
+  double wt = 0.0, unused;
+  uint32_t ct = 0;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    wt += (double)m[j] * unit;
+    ct += c[j];
+  }
+  double before_w = block_scan<kSliceWaves>(wt, s.wave_d, unused) - wt;
+  uint32_t before_c = block_scan_u<kSliceWaves>(ct, s.wave_u) - ct;
+  if (tid == 0) s.bin = kSliceBins;
+  __syncthreads();
+  {
+    double run = before_w;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      run += (double)m[j] * unit;
+      if (c[j] > 0 && run >= target) {
+        atomicMin(&s.bin, tid * PER + j);
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  int lo = s.bin, hi = s.bin;
+  if (lo < kSliceBins && q.min_p > 0.0) {
+    // where w = min_p, give or take the bins' rounding
+    const double at = -log2(q.min_p) / weight.per * (double)weight.bins * 0.5;
+    const int b = at < (double)kSliceBins ? (int)at : kSliceBins;
+    if (b + 1 < lo) {
+      lo = max(b - 1, 0);
+      hi = b + 1;
+    } else if (b - 1 <= hi) {
+      lo = max(min(lo, b - 1), 0);
+    }
+  }
+  // the tokens in them, and what lies before
+  if (tid == 0) s.n = 0;
+  if (tid == lo / PER && lo < kSliceBins) {
+    double w = before_w;
+    uint32_t n = before_c;
+    for (int j = 0; j < PER && tid * PER + j < lo; j++) {
+      w += (double)m[j] * unit;
+      n += c[j];
+    }
+    sa.info[r].below = w;
+    sa.info[r].before = n;
+  }
+  __syncthreads();
+  uint32_t in = 0;
+#pragma unroll
+  for (int j = 0; j < PER; j++)
+    if (tid * PER + j >= lo && tid * PER + j <= hi) in += c[j];
+  if (in > 0) atomicAdd(&s.n, in);
+  __syncthreads();
+  if (tid == 0) {
+    sa.info[r].lo = lo < kSliceBins && s.n <= (uint32_t)kList ? lo : -1;
+    sa.info[r].hi = hi;
+    sa.info[r].all = all;
+  }
+}
+
+template <class E>
+__global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SliceArgs sa) {
+  __shared__ SliceLds s;
+  const int r = blockIdx.y, sl = blockIdx.x, tid = threadIdx.x;
+  const RowParams q(sa.a, r);
+  if (q.way != Way::kTopK && q.way != Way::kNucleus) return;
+  float top;
+  int first;
+  row_top(sa, r, top, first);
+  if (first < 0) return;
+  const SliceInfo info = sa.info[r];
+  if (q.way == Way::kNucleus && info.lo < 0) return;
+  const SliceView<E> view(sa, r, sl);
+  const size_t rs = (size_t)r * sa.S + sl;
+  const Weight weight = nucleus_weight(q, top, sa.a.V);
+  const double least = q.least(sa.a.V);
+  if (tid == 0) s.n = 0;
+  __syncthreads();
+  auto keep = [&](float v, int i) {
+    const uint32_t n = atomicAdd(&s.n, 1u);
+    if (n < kList) sa.list[rs * kList + n] = make_uint2(key_of(v), (uint32_t)i);
+  };
+  if (q.way == Way::kTopK) {
+    view.row.walk(view.w0, view.w1, [&](float v, int i) {
+      if (v >= info.cut) keep(v, i);
+    });
+  } else {
+    view.row.walk(view.w0, view.w1, [&](float v, int i) {
+      const int b = weight.bin(v);
+      if (b >= info.lo && b <= info.hi && weight.of(v) >= least) keep(v, i);
+    });
+    // the slice's weight before the bins
+    double x = 0.0, below;
+    const double unit = 1.0 / fixed_point(sa.a.V);
+    for (int i = tid; i < info.lo; i += kSliceThreads)
+      x += (double)sa.mass[rs * kSliceBins + i] * unit;
+    block_scan<kSliceWaves>(x, s.wave_d, below);
+    if (tid == 0) sa.total[rs] = below;
+  }
+  __syncthreads();
+  if (tid == 0) sa.listed[rs] = s.n;
+}
+
+// The row's lists into s.key / s.index in index order; their number, or kList + 1
+// for more than fit.  s.upto[i]: tokens of slices 0 .. i.
+__device__ __forceinline__ int join_lists(const SliceArgs& sa, int r, Lds& s) {
+  const int lane = threadIdx.x & 63;
+  const size_t r0 = (size_t)r * sa.S;
+  uint32_t n = lane < sa.S ? sa.listed[r0 + lane] : 0;
+  const bool over = __builtin_amdgcn_ballot_w64(n > (uint32_t)kList) != 0;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t y = __shfl_up(n, d, 64);
+    if (lane >= d) n += y;
+  }
+  const uint32_t total = __shfl(n, 63, 64);
+  __syncthreads();
+  if (threadIdx.x < 64) s.upto[lane] = n;
+  __syncthreads();
+  if (over || total > (uint32_t)kList) return kList + 1;
+  const uint32_t i = threadIdx.x;
+  if (i < total) {
+    int sl = 0;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+      if (s.upto[sl + d - 1] <= i) sl += d;
+    const uint2 e = sa.list[(r0 + sl) * kList + (i - (sl > 0 ? s.upto[sl - 1] : 0))];
+    s.key2[i] = e.x;
+    s.index2[i] = (int)e.y;
+  }
+  __syncthreads();
+  sort_list(s, (int)total);
+  return (int)total;
+}
+
+// A row's own workgroup: the whole row, or with SLICED what its slices leave.
+template <class E, bool SLICED>
+__global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
   __shared__ Lds s;
+  const SampleArgs& a = sa.a;
   const int r = blockIdx.x;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const RowView<E> row(a.logits, r * a.row_stride, a.V);
   const int per = (row.vectors + kWaves - 1) / kWaves;
   const int w0 = min(wave * per, row.vectors), w1 = min((wave + 1) * per, row.vectors);
-  const float T = a.temperature ? a.temperature[r] : 1.f;
-  const double u = a.u[r];
-  const int k = a.top_k ? a.top_k[r] : 0;
-  const float p = a.top_p ? a.top_p[r] : 1.f;
-  const double min_p = a.min_p && a.min_p[r] > 0.f ? fmin((double)a.min_p[r], 1.0) : 0.0;
+  const RowParams q(a, r);
 
   // ---- the max, and its first index
   float mine = -INFINITY;
-  int at = -1;
-  row.walk(w0, w1, [&](float v, int i) {
-    if (v > mine) {
-      mine = v;
-      at = i;
-    }
-  });
-  {
-    float x = mine;
-    int i = at;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      const float y = __shfl_xor(x, d, 64);
-      const int j = __shfl_xor(i, d, 64);
-      if (y > x || (y == x && (uint32_t)j < (uint32_t)i)) {
-        x = y;
-        i = j;
+  Weight weight;
+  int first;
+  if constexpr (SLICED) {
+    row_top(sa, r, weight.top, first);
+  } else {
+    int at = -1;
+    row.walk(w0, w1, [&](float v, int i) {
+      if (v > mine) {
+        mine = v;
+        at = i;
       }
-    }
+    });
+    float x = mine;
+    wave_top(x, at);
     if (lane == 0) {
       s.wave_f[wave] = x;
-      s.wave_i[wave] = i;
+      s.wave_i[wave] = at;
     }
-  }
-  __syncthreads();
-  Weight weight;
-  weight.top = s.wave_f[0];
-  int first = s.wave_i[0];
+    __syncthreads();
+    weight.top = s.wave_f[0];
+    first = s.wave_i[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; w++)
-    if (s.wave_f[w] > weight.top) {
-      weight.top = s.wave_f[w];
-      first = s.wave_i[w];
-    }
-  const bool hot = T >= kMinTemperature;
-  if (first < 0 || !hot) {  // nothing to draw from, or the max itself
+    for (int w = 1; w < kWaves; w++)
+      if (s.wave_f[w] > weight.top) {
+        weight.top = s.wave_f[w];
+        first = s.wave_i[w];
+      }
+  }
+  if (first < 0 || q.way == Way::kTop) {  // nothing to draw from, or the max itself
     if (threadIdx.x == 0) {
       a.tokens[r] = first;
       if (a.probs) a.probs[r] = first < 0 ? 0.f : 1.f;
     }
     return;
   }
-  weight.per = 1.4426950408889634 / (double)T;
+  weight.per = 1.4426950408889634 / (double)q.T;
   weight.bins = 2.f * kBinsPerLog2 * (float)weight.per;
-  const bool has_k = k > 0 && k < a.V;
-  const bool has_p = p < 1.f;
-  // fixed point of the histogram's weights: V of them fit 63 bits
-  const double fixed = ldexp(1.0, 30 + __clz(a.V));
+  weight.limit = kBins;
+  const double fixed = fixed_point(a.V);
 
   int token = -1;
   double w_token = 0.0, total = 0.0;
   int n = kList + 1;      // listed tokens
-  double all = 0.0;       // the total that top-p is a share of (has_k: the list's)
-  if (has_k && k <= kList) {
+  double all = 0.0;       // the total that top-p is a share of (top-k: the list's)
+  double below = 0.0;     // weight and
+  uint32_t before = 0;    // number of the tokens before the listed
+  bool slices = false;    // the row's weight is in its slices, the list only its last part
+  if constexpr (SLICED) {
+    if (q.way == Way::kTopK) {
+      n = join_lists(sa, r, s);
+    } else if (q.way == Way::kNucleus) {
+      const SliceInfo info = sa.info[r];
+      if (info.lo >= 0) {
+        n = join_lists(sa, r, s);
+        all = info.all;
+        below = info.below;
+        before = info.before;
+        slices = n <= kList && before > 0;
+      }
+    } else if (q.way == Way::kTotals) {
+      n = 0;
+      slices = true;
+    }
+  } else if (q.way == Way::kTopK) {
     // the k-th largest of the threads' maxima, to a bin
     clear_histogram(s);
     const int b = weight.bin(mine);
     if (b < kBins) atomicAdd(&s.count[b], 1u);
     __syncthreads();
-    const int cut = find_bin<true>(s, (uint32_t)k, 0.0, 0.0).bin;
+    const int cut = find_bin<true>(s, (uint32_t)q.k, 0.0, 0.0).bin;
     // (kBins: fewer than k threads hold a token of weight)
     n = gather(row, s, [&](float v, int) { return weight.bin(v) <= min(cut, kBins - 1); });
-  } else if (has_p && !has_k) {
-    const double least = 0.5 * fmax(1.0 - (double)p, 0.0) / (double)a.V;
+  } else if (q.way == Way::kNucleus) {
+    const double least = q.least(a.V);
     clear_histogram(s);
     double x = 0.0;
     row.walk(w0, w1, [&](float v, int) {
@@ -664,15 +1153,18 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       }
     });
     block_scan(x, s.wave_d, all);
-    // (a little beyond p: the fixed-point sums are cut off)
-    const BinAt b = find_bin<false>(s, 0, (double)p * all * (1.0 + 1e-9), 1.0 / fixed);
+    // (a little beyond p: the fixed-point sums are rounded)
+    const BinAt b = find_bin<false>(s, 0, (double)q.p * all * (1.0 + 1e-9), 1.0 / fixed);
     if (b.bin < kBins && b.before + b.in <= (uint32_t)kList)
       n = gather(row, s, [&](float v, int) { return weight.bin(v) <= b.bin; });
   }
   if (n <= kList) {
     const int i = threadIdx.x;
     if (i < n) s.weight[i] = weight.of(value_of_key(s.key[i]));
-    if (i == 0) s.found = kList;
+    if (i == 0) {
+      s.found = kList;
+      s.lo = 0;
+    }
     __syncthreads();
     uint32_t rank = 0;
     double above = 0.0, w = 0.0;
@@ -680,37 +1172,87 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     if (in) {
       rank_of(s, n, i, rank, above);
       w = s.weight[i];
-      if (has_k) in = rank < (uint32_t)k;
+      if (q.has_k) in = rank < (uint32_t)q.k;
     }
-    if (has_k && has_p) block_scan(in ? w : 0.0, s.wave_d, all);
-    if (in && has_p) in = above < (double)p * all || rank == 0;
-    if (in) in = w >= min_p;
-    const double upto = block_scan(in ? w : 0.0, s.wave_d, total);
-    const double target = u * total;
-    if (in && upto > target) atomicMin(&s.found, i);
-    __syncthreads();
-    if (s.found == kList) {  // u at or above 1 (or rounding): the last kept
+    if (q.has_k && q.has_p) block_scan(in ? w : 0.0, s.wave_d, all);
+    if (in && q.has_p) in = below + above < (double)q.p * all || rank + before == 0;
+    if (in) in = w >= q.min_p;
+    if (!slices) {
+      const double upto = block_scan(in ? w : 0.0, s.wave_d, total);
+      const double target = q.u * total;
+      if (in && upto > target) atomicMin(&s.found, i);
       __syncthreads();
-      if (i == 0) s.found = -1;
+      if (s.found == kList) {  // u at or above 1 (or rounding): the last kept
+        __syncthreads();
+        if (i == 0) s.found = -1;
+        __syncthreads();
+        if (in) atomicMax(&s.found, i);
+        __syncthreads();
+      }
+      token = s.index[s.found];
+      w_token = s.weight[s.found];
+    } else {
+      // The last kept token of the list, and with it the slices' weights.
+      if (in) {
+        atomicMax(&s.lo, rank + 1);
+        s.index2[rank] = i;
+      }
+      if (i < n) s.weight[i] = in ? w : 0.0;
       __syncthreads();
-      if (in) atomicMax(&s.found, i);
+      Kept kept;  // (of the list; none of it, where none of it is kept)
+      kept.key = 0xFFFFFFFFu;
+      kept.last = -1;
+      if (s.lo > 0) {
+        const int e = s.index2[s.lo - 1];
+        kept.key = s.key[e];
+        kept.last = s.index[e];
+      }
+      const bool totals = q.way == Way::kTotals;
+      if (i < sa.S) {
+        double x = sa.total[(size_t)r * sa.S + i];
+        if (!totals)
+          for (uint32_t j = i > 0 ? s.upto[i - 1] : 0; j < s.upto[i]; j++) x += s.weight[j];
+        s.slice_w[i] = x;
+      }
       __syncthreads();
+      for (int j = 0; j < sa.S; j++) total += s.slice_w[j];
+      const double target = q.u * total;
+      int at = -1;
+      double base = 0.0, run = 0.0;
+      for (int j = 0; j < sa.S; j++) {
+        const double x = s.slice_w[j];
+        // (the last slice with weight takes what rounding leaves over)
+        if (x > 0.0 && (at < 0 || !(run > target))) {
+          at = j;
+          base = run;
+        }
+        run += x;
+      }
+      const int sp = (row.vectors + sa.S - 1) / sa.S;
+      const int v0 = min(max(at, 0) * sp, row.vectors), v1 = min(v0 + sp, row.vectors);
+      const Weight bins = nucleus_weight(q, weight.top, a.V);
+      const int lo = totals ? 0 : sa.info[r].lo;
+      const Found f = find_within(row, v0, v1, base, target, s, [&](float v, int idx) {
+        const double y = weight.of(v);
+        if (totals) return y >= q.min_p ? y : 0.0;
+        return bins.bin(v) < lo || kept.has(key_of(v), idx) ? y : 0.0;
+      });
+      token = f.index;
+      w_token = f.f;
     }
-    token = s.index[s.found];
-    w_token = s.weight[s.found];
   } else {
     Kept kept;
-    if (has_k) kept = last_kept<true>(row, weight, kept, (uint32_t)k, 0.0, fixed, s);
-    if (has_p) {
+    if (q.has_k) kept = last_kept<true>(row, weight, kept, (uint32_t)q.k, 0.0, fixed, s);
+    if (q.has_p) {
       double x = 0.0;
       row.walk(w0, w1, [&](float v, int i) { x += kept.has(key_of(v), i) ? weight.of(v) : 0.0; });
       block_scan(x, s.wave_d, all);
-      kept = last_kept<false>(row, weight, kept, 0u, (double)p * all, fixed, s);
+      kept = last_kept<false>(row, weight, kept, 0u, (double)q.p * all, fixed, s);
     }
-    const Found f = find_index<true>(row, u, s, [&](float v, int i) {
+    const Found f = find_index<true>(row, q.u, s, [&](float v, int i) {
       if (!kept.has(key_of(v), i)) return 0.0;
       const double w = weight.of(v);
-      return w >= min_p ? w : 0.0;
+      return w >= q.min_p ? w : 0.0;
     });
     token = f.index;
     w_token = f.f;
@@ -722,13 +1264,78 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   }
 }
 
+// ---- launch ------------------------------------------------------------------
+
+struct Layout {
+  int S = 1;  // 1: no slices
+  size_t thread_top = 0, first = 0, total = 0, mass = 0, count = 0, listed = 0, list = 0, info = 0,
+         arrived = 0, bytes = 0;
+};
+
+// Some 1024 slices over all rows, of 4096 tokens or more.
+Layout layout_of(int rows, int V) {
+  Layout l;
+  int64_t S = (1024 + (int64_t)rows - 1) / rows;
+  S = S < V / 4096 ? S : V / 4096;
+  S = S < kMaxSlices ? S : kMaxSlices;
+  if (S < 2) return l;
+  l.S = (int)S;
+  const size_t n = (size_t)rows * S;
+  size_t at = 0;
+  auto put = [&](size_t bytes) {
+    const size_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  put(n * 4);  // top
+  l.first = put(n * 4);
+  l.thread_top = put(n * 4 * kSliceThreads);
+  l.total = put(n * 8);
+  l.mass = put(n * 8 * kSliceBins);
+  l.count = put(n * 4 * kSliceBins);
+  l.listed = put(n * 4);
+  l.list = put(n * 8 * kList);
+  l.info = put((size_t)rows * sizeof(SliceInfo));
+  l.arrived = put((size_t)rows * 4);
+  l.bytes = at;
+  return l;
+}
+
+template <class E>
+int launch_sample(const SliceArgs& sa, int rows, hipStream_t st) {
+  if (sa.S < 2) {
+    sample_kernel<E, false><<<dim3(rows), dim3(kThreads), 0, st>>>(sa);
+    return launch_status();
+  }
+  const dim3 grid(sa.S, rows), block(kSliceThreads);
+  sample_max_kernel<E><<<grid, block, 0, st>>>(sa);
+  int s = launch_status();
+  if (s != SDE_OK) return s;
+  sample_weights_kernel<E><<<grid, block, 0, st>>>(sa);
+  s = launch_status();
+  if (s != SDE_OK) return s;
+  sample_gather_kernel<E><<<grid, block, 0, st>>>(sa);
+  s = launch_status();
+  if (s != SDE_OK) return s;
+  sample_kernel<E, true><<<dim3(rows), dim3(kThreads), 0, st>>>(sa);
+  return launch_status();
+}
+
 }  // namespace smp
 }  // namespace sde
 
-extern "C" int sde_sample(const void* d_logits, int64_t row_stride, int dtype, int n_rows,
-                          int vocab, const float* d_u, const float* d_temperature,
-                          const int32_t* d_top_k, const float* d_top_p, const float* d_min_p,
-                          int32_t* d_tokens, float* d_probs, sde_stream_t stream) {
+extern "C" {
+
+size_t sde_sample_workspace_size(int n_rows, int vocab) {
+  using namespace sde::smp;
+  if (n_rows < 1 || vocab < 1 || vocab > kMaxVocab || n_rows > (1 << 21)) return 0;
+  return layout_of(n_rows, vocab).bytes;
+}
+
+int sde_sample(const void* d_logits, int64_t row_stride, int dtype, int n_rows, int vocab,
+               const float* d_u, const float* d_temperature, const int32_t* d_top_k,
+               const float* d_top_p, const float* d_min_p, int32_t* d_tokens, float* d_probs,
+               void* d_workspace, size_t workspace_bytes, sde_stream_t stream) {
   using namespace sde::smp;
   if (n_rows < 0 || vocab < 1 || !sde::batch::known_dtype(dtype)) return SDE_ERR_INVALID_ARGUMENT;
   if (vocab > kMaxVocab || n_rows > (1 << 21)) return SDE_ERR_UNSUPPORTED;
@@ -737,14 +1344,31 @@ extern "C" int sde_sample(const void* d_logits, int64_t row_stride, int dtype, i
     return SDE_ERR_INVALID_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(d_logits) % (size_t)sde::batch::elem_bytes(dtype) != 0)
     return SDE_ERR_INVALID_ARGUMENT;
-  const SampleArgs a{d_logits, row_stride, vocab,   d_u,      d_temperature,
-                     d_top_k,  d_top_p,    d_min_p, d_tokens, d_probs};
+  const Layout l = layout_of(n_rows, vocab);
+  if (l.bytes > 0 && (!d_workspace || workspace_bytes < l.bytes ||
+                      reinterpret_cast<uintptr_t>(d_workspace) % 16 != 0))
+    return SDE_ERR_WORKSPACE;
+  SliceArgs sa{};
+  sa.a = SampleArgs{d_logits, row_stride, vocab,   d_u,      d_temperature,
+                    d_top_k,  d_top_p,    d_min_p, d_tokens, d_probs};
+  sa.S = l.S;
+  if (l.S > 1) {
+    char* w = static_cast<char*>(d_workspace);
+    sa.top = reinterpret_cast<float*>(w);
+    sa.first = reinterpret_cast<int*>(w + l.first);
+    sa.thread_top = reinterpret_cast<float*>(w + l.thread_top);
+    sa.total = reinterpret_cast<double*>(w + l.total);
+    sa.mass = reinterpret_cast<unsigned long long*>(w + l.mass);
+    sa.count = reinterpret_cast<uint32_t*>(w + l.count);
+    sa.listed = reinterpret_cast<uint32_t*>(w + l.listed);
+    sa.list = reinterpret_cast<uint2*>(w + l.list);
+    sa.info = reinterpret_cast<SliceInfo*>(w + l.info);
+    sa.arrived = reinterpret_cast<uint32_t*>(w + l.arrived);
+  }
   const hipStream_t s = (hipStream_t)stream;
-  if (dtype == SDE_F32)
-    sample_kernel<sde::batch::f32_elem><<<dim3(n_rows), dim3(kThreads), 0, s>>>(a);
-  else if (dtype == SDE_F16)
-    sample_kernel<sde::batch::f16_elem><<<dim3(n_rows), dim3(kThreads), 0, s>>>(a);
-  else
-    sample_kernel<sde::batch::bf16_elem><<<dim3(n_rows), dim3(kThreads), 0, s>>>(a);
-  return sde::launch_status();
+  if (dtype == SDE_F32) return launch_sample<sde::batch::f32_elem>(sa, n_rows, s);
+  if (dtype == SDE_F16) return launch_sample<sde::batch::f16_elem>(sa, n_rows, s);
+  return launch_sample<sde::batch::bf16_elem>(sa, n_rows, s);
 }
+
+}  // extern "C"

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from conftest import case_banner
-from speculative_decode_engine_amd import SDEError, sample
+from speculative_decode_engine_amd import SDEError, sample, sample_workspace_size
 
 pytestmark = pytest.mark.gpu
 
@@ -234,8 +234,17 @@ def test_refusals(gpu):
             (dict(top_p=u.int()), TypeError), (dict(min_p=u.cpu()), TypeError),
             (dict(temperature=u[:1]), ValueError), (dict(tokens=u), TypeError),
             (dict(probs=u[::2]), ValueError),
+            (dict(workspace=torch.zeros(9)), ValueError),
             (dict(logits=torch.zeros(3, 0, device="cuda")), (ValueError, SDEError))]:
         args = dict(logits=x, u=u)
         args.update(bad)
         with pytest.raises(error):
             sample(**args)
+    y = torch.zeros(2, 32000, device="cuda")
+    need = sample_workspace_size(2, 32000)
+    assert need > 0 and sample_workspace_size(2, 50) == 0
+    ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    sample(y, u[:2], workspace=ws)
+    with pytest.raises(SDEError) as e:
+        sample(y, u[:2], workspace=ws[:-16])
+    assert e.value.status == 5

@@ -49,7 +49,7 @@ constexpr int kList = 512;            // tokens compared in LDS
 constexpr int kSliceThreads = 256;    // of a slice's workgroup
 constexpr int kSliceWaves = kSliceThreads / 64;
 constexpr int kSliceBins = 1024;
-constexpr int kMaxSlices = 64;
+constexpr int kMaxSlices = 16;
 constexpr float kMinTemperature = 1e-6f;
 constexpr int kMaxVocab = 1 << 24;
 
@@ -76,10 +76,10 @@ __device__ __forceinline__ float value_of_key(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// 2^t for t <= 0, to 1e-14 of it: the integer part to the exponent, the rest
-// f in [-1/2, 1/2] by the series of exp(f ln 2).
+// 2^t for t <= 0, to 1e-14 of it, and 0 from -1100 down: the integer part to the
+// exponent, the rest f in [-1/2, 1/2] by the series of exp(f ln 2).
 __device__ __forceinline__ double exp2_f64(double t) {
-  if (t < -1000.0) return 0.0;
+  t = fmax(t, -1100.0);
   const double n = rint(t);
   const double f = t - n;
   double y = 4.44553827187081e-10;  // ln(2)^11 / 11!
@@ -104,9 +104,9 @@ struct Weight {
   float bins;     // histogram bins per unit of (max - x) / 2
   int limit;      // and their number
   __device__ __forceinline__ double of(float x) const {
-    if (x == top) return 1.0;
-    if (x == -INFINITY) return 0.0;
-    return exp2_f64(((double)x - (double)top) * per);
+    // (NaN where an infinite T meets -inf: 0, as its -1100)
+    const double w = exp2_f64(((double)x - (double)top) * per);
+    return x == top ? 1.0 : w;
   }
   // 0 at the max, rising as x falls; `limit`: left out
   __device__ __forceinline__ int bin(float x) const {
@@ -187,11 +187,11 @@ struct RowView {
 struct Lds {
   uint32_t count[kBins];
   unsigned long long mass[kBins];
-  uint32_t key[kList];
+  __attribute__((aligned(16))) uint32_t key[kList];
   int index[kList];
-  double weight[kList];
+  __attribute__((aligned(16))) double weight[kList];
   uint32_t key2[kList];
-  int index2[kList];
+  __attribute__((aligned(16))) int index2[kList];
   double wave_d[kWaves];
   double wave_d2[kWaves];
   uint32_t wave_u[kWaves];
@@ -440,13 +440,21 @@ __device__ __forceinline__ Found find_index(const RowView<E>& row, double share,
   return r;
 }
 
-// s.key2 / s.index2 to s.key / s.index in index order.
+// s.key2 / s.index2 to s.key / s.index in index order.  (Four listed tokens a
+// read here and below: the loops run at the LDS latency otherwise.)
 __device__ __forceinline__ void sort_list(Lds& s, int n) {
-  if ((int)threadIdx.x < n) {
-    const int me = s.index2[threadIdx.x];
+  const int i = threadIdx.x;
+  if (i >= n && i < (n + 3) / 4 * 4) s.index2[i] = INT32_MAX;
+  __syncthreads();
+  if (i < n) {
+    const int me = s.index2[i];
     int at = 0;
-    for (int j = 0; j < n; j++) at += s.index2[j] < me ? 1 : 0;
-    s.key[at] = s.key2[threadIdx.x];
+#pragma unroll 4
+    for (int j = 0; j < n; j += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(&s.index2[j]);
+      at += (o.x < me) + (o.y < me) + (o.z < me) + (o.w < me);
+    }
+    s.key[at] = s.key2[i];
     s.index[at] = me;
   }
   __syncthreads();
@@ -477,17 +485,35 @@ __device__ __forceinline__ int gather(const RowView<E>& row, Lds& s, P in) {
   return (int)n;
 }
 
+// The listed tokens' weights to s.weight, and the list filled up to a multiple
+// of four with tokens before which every other comes.  Every thread calls it.
+__device__ __forceinline__ void weigh_list(Lds& s, int n, const Weight& weight) {
+  const int i = threadIdx.x;
+  if (i < (n + 3) / 4 * 4) {
+    if (i >= n) s.key[i] = 0;
+    s.weight[i] = i < n ? weight.of(value_of_key(s.key[i])) : 0.0;
+  }
+  __syncthreads();
+}
+
 // Rank of listed token i among the n listed (falling value, rising index) and
 // the weight of those before it.
 __device__ __forceinline__ void rank_of(const Lds& s, int n, int i, uint32_t& rank, double& above) {
   const uint32_t k = s.key[i];
   uint32_t r = 0;
   double a = 0.0;
-  for (int j = 0; j < n; j++) {
-    const uint32_t o = s.key[j];
-    const bool first = o > k || (o == k && j < i);
-    r += first ? 1u : 0u;
-    a += first ? s.weight[j] : 0.0;
+#pragma unroll 2
+  for (int j = 0; j < n; j += 4) {
+    const uint4 o = *reinterpret_cast<const uint4*>(&s.key[j]);
+    const double2 w0 = *reinterpret_cast<const double2*>(&s.weight[j]);
+    const double2 w1 = *reinterpret_cast<const double2*>(&s.weight[j + 2]);
+    const bool b0 = o.x > k || (o.x == k && j < i), b1 = o.y > k || (o.y == k && j + 1 < i);
+    const bool b2 = o.z > k || (o.z == k && j + 2 < i), b3 = o.w > k || (o.w == k && j + 3 < i);
+    r += (uint32_t)b0 + b1 + b2 + b3;
+    a += b0 ? w0.x : 0.0;
+    a += b1 ? w0.y : 0.0;
+    a += b2 ? w1.x : 0.0;
+    a += b3 ? w1.y : 0.0;
   }
   rank = r;
   above = a;
@@ -532,9 +558,8 @@ __device__ __forceinline__ Kept last_kept(const RowView<E>& row, const Weight& w
     if (at.in <= (uint32_t)kList) {
       const int n = gather(row, s, inside);
       const int i = threadIdx.x;
-      if (i < n) s.weight[i] = weight.of(value_of_key(s.key[i]));
       if (i == 0) s.found = -1;
-      __syncthreads();
+      weigh_list(s, n, weight);
       if (i < n) {
         uint32_t rank;
         double above;
@@ -603,18 +628,21 @@ __device__ __forceinline__ Kept last_kept(const RowView<E>& row, const Weight& w
 // needed.  With fewer rows than fill the chip, a row is cut into slices of
 // vectors, a workgroup each, in three launches before the row's own:
 //  max      the slice's max, and each thread's for top-k;
-//  weights  top-k: the cut, a bound of the k-th largest (one workgroup a row);
-//           top-p: the slice's total and histogram; the last workgroup of a row
-//           joins them and finds the bin that holds the last kept token;
+//  weights  top-k up to kList: the cut, a bound of the k-th largest (one
+//           workgroup a row);
+//           a larger k, or top-p: the slice's histogram, of tokens or of weight,
+//           and its total; the last workgroup of a row joins them and finds the
+//           bin that holds the last kept token;
 //           neither: the slice's total;
 //  gather   the tokens at or above the cut, or in that bin, into a list per
 //           slice, and the slice's weight before the bin.
 // The row's workgroup then has the lists to compare, and the slices' weights
 // to find the one that holds the token, which alone it walks.
 // Which way a row goes is told by its parameters; one whose list would be too
-// long (flat rows, ties, k above kList) is walked whole by its workgroup.
+// long (flat rows, ties), or with both a large k and top-p, is walked whole by
+// its workgroup.
 
-enum class Way { kTop, kTopK, kNucleus, kTotals, kWhole };
+enum class Way { kTop, kTopK, kRank, kNucleus, kTotals, kWhole };
 
 struct RowParams {
   float T, p;
@@ -633,7 +661,7 @@ struct RowParams {
     if (!(T >= kMinTemperature))
       way = Way::kTop;
     else if (has_k)
-      way = k <= kList ? Way::kTopK : Way::kWhole;
+      way = k <= kList ? Way::kTopK : has_p ? Way::kWhole : Way::kRank;
     else
       way = has_p ? Way::kNucleus : Way::kTotals;
   }
@@ -649,10 +677,9 @@ __device__ __forceinline__ double fixed_point(int V) { return ldexp(1.0, 30 + __
 
 struct SliceInfo {  // of a row
   float cut;        // top-k: the lowest value listed
-  int lo, hi;       // top-p: the bins listed (lo < 0: none could be told)
-  uint32_t before;  // tokens before them
-  double below;     // and their weight
-  double all;       // the row's
+  int lo, hi;       // the bins listed
+  double below;     // what lies before them: weight (tokens, where top-k acts)
+  double all;       // the row's weight
 };
 
 struct SliceArgs {
@@ -662,8 +689,7 @@ struct SliceArgs {
   int* first;                 // [rows][S]
   float* thread_top;          // [rows][S][kSliceThreads]
   double* total;              // [rows][S]; after the gather: the weight before bin lo
-  unsigned long long* mass;   // [rows][S][kSliceBins]
-  uint32_t* count;            // [rows][S][kSliceBins]
+  unsigned long long* mass;   // [rows][S][kSliceBins] (tokens, where top-k acts)
   uint32_t* listed;           // [rows][S]
   uint2* list;                // [rows][S][kList]: key, index
   SliceInfo* info;            // [rows]
@@ -671,7 +697,6 @@ struct SliceArgs {
 };
 
 struct SliceLds {
-  uint32_t count[kSliceBins];
   unsigned long long mass[kSliceBins];
   double wave_d[kSliceWaves];
   uint32_t wave_u[kSliceWaves];
@@ -725,12 +750,13 @@ __device__ __forceinline__ void row_top(const SliceArgs& sa, int r, float& x, in
 }
 
 // The bins of a nucleus: from the max down to the least weight that can be its
-// last.
-__device__ __forceinline__ Weight nucleus_weight(const RowParams& q, float top, int V) {
+// last.  Of a larger k's: 2^-64 of the max, below which nothing is drawn.
+__device__ __forceinline__ Weight slice_weight(const RowParams& q, float top, int V) {
   Weight w;
   w.top = top;
   w.per = 1.4426950408889634 / (double)q.T;
-  const float range = log2f((float)V / (1.f - fmaxf(q.p, 0.f))) + 2.f;
+  const float range =
+      q.way == Way::kNucleus ? log2f((float)V / (1.f - fmaxf(q.p, 0.f))) + 2.f : 64.f;
   w.bins = 2.f * (float)w.per * ((float)kSliceBins / range);
   w.limit = kSliceBins;
   return w;
@@ -774,9 +800,14 @@ __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SliceArgs sa)
 // width): at least k tokens do.
 __device__ __forceinline__ float top_k_cut(const SliceArgs& sa, int r, int k, float top,
                                            SliceLds& s) {
-  const int tid = threadIdx.x, n = sa.S * kSliceThreads;
-  const float* t = sa.thread_top + (size_t)r * n;
-  for (int i = tid; i < kSliceBins; i += kSliceThreads) s.count[i] = 0;
+  const int tid = threadIdx.x;
+  const float* t = sa.thread_top + (size_t)r * sa.S * kSliceThreads + tid;
+  float x[kMaxSlices];
+#pragma unroll
+  for (int i = 0; i < kMaxSlices; i++)
+    x[i] = i < sa.S ? t[(size_t)i * kSliceThreads] : -INFINITY;
+  uint32_t* const count = reinterpret_cast<uint32_t*>(s.mass);
+  for (int i = tid; i < kSliceBins; i += kSliceThreads) count[i] = 0;
   if (tid == 0) {
     s.key = 0xFFFFFFFFu;
     s.bin = kSliceBins;
@@ -785,13 +816,12 @@ __device__ __forceinline__ float top_k_cut(const SliceArgs& sa, int r, int k, fl
   __syncthreads();
   float low = INFINITY;
   uint32_t live = 0;
-  for (int i = tid; i < n; i += kSliceThreads) {
-    const float x = t[i];
-    if (x > -INFINITY) {
-      low = fminf(low, x);
+#pragma unroll
+  for (int i = 0; i < kMaxSlices; i++)
+    if (x[i] > -INFINITY) {
+      low = fminf(low, x[i]);
       live++;
     }
-  }
   if (live > 0) {
     atomicMin(&s.key, key_of(low));
     atomicAdd(&s.n, live);
@@ -801,20 +831,21 @@ __device__ __forceinline__ float top_k_cut(const SliceArgs& sa, int r, int k, fl
   low = value_of_key(s.key);
   const float span = 0.5f * top - 0.5f * low;
   const float scale = span > 0.f && span < INFINITY ? (float)(kSliceBins - 1) / span : 0.f;
-  auto bin = [&](float x) {
-    return x == top ? 0 : (int)fminf((0.5f * top - 0.5f * x) * scale, (float)(kSliceBins - 1));
+  auto bin = [&](float v) {
+    return v == top ? 0 : (int)fminf((0.5f * top - 0.5f * v) * scale, (float)(kSliceBins - 1));
   };
-  for (int i = tid; i < n; i += kSliceThreads) {
-    const float x = t[i];
-    if (x > -INFINITY) atomicAdd(&s.count[bin(x)], 1u);
-  }
+#pragma unroll
+  for (int i = 0; i < kMaxSlices; i++)
+    if (x[i] > -INFINITY) atomicAdd(&count[bin(x[i])], 1u);
   __syncthreads();
   constexpr int PER = kSliceBins / kSliceThreads;
   uint32_t c = 0;
-  for (int i = 0; i < PER; i++) c += s.count[tid * PER + i];
+#pragma unroll
+  for (int i = 0; i < PER; i++) c += count[tid * PER + i];
   uint32_t run = block_scan_u<kSliceWaves>(c, s.wave_u) - c;
+#pragma unroll
   for (int i = 0; i < PER; i++) {
-    run += s.count[tid * PER + i];
+    run += count[tid * PER + i];
     if (run >= (uint32_t)k) {
       atomicMin(&s.bin, tid * PER + i);
       break;
@@ -824,10 +855,9 @@ __device__ __forceinline__ float top_k_cut(const SliceArgs& sa, int r, int k, fl
   __syncthreads();
   const int b = s.bin;
   low = INFINITY;
-  for (int i = tid; i < n; i += kSliceThreads) {
-    const float x = t[i];
-    if (x > -INFINITY && bin(x) <= b) low = fminf(low, x);
-  }
+#pragma unroll
+  for (int i = 0; i < kMaxSlices; i++)
+    if (x[i] > -INFINITY && bin(x[i]) <= b) low = fminf(low, x[i]);
   if (low < INFINITY) atomicMin(&s.key, key_of(low));
   __syncthreads();
   return s.key == 0xFFFFFFFFu ? top : value_of_key(s.key);
@@ -850,7 +880,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs
   }
   const SliceView<E> view(sa, r, sl);
   const size_t rs = (size_t)r * sa.S + sl;
-  const Weight weight = nucleus_weight(q, top, sa.a.V);
+  const Weight weight = slice_weight(q, top, sa.a.V);
   double x = 0.0, all;
   if (q.way == Way::kTotals) {
     view.row.walk(view.w0, view.w1, [&](float v, int) {
@@ -861,30 +891,30 @@ __global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs
     if (tid == 0) sa.total[rs] = all;
     return;
   }
-  const double fixed = fixed_point(sa.a.V), least = q.least(sa.a.V);
-  for (int i = tid; i < kSliceBins; i += kSliceThreads) {
-    s.count[i] = 0;
-    s.mass[i] = 0;
-  }
+  for (int i = tid; i < kSliceBins; i += kSliceThreads) s.mass[i] = 0;
   __syncthreads();
-  view.row.walk(view.w0, view.w1, [&](float v, int) {
-    const double w = weight.of(v);
-    x += w;
-    const int b = weight.bin(v);
-    if (w >= least && b < kSliceBins) {
-      atomicAdd(&s.count[b], 1u);
-      atomicAdd(&s.mass[b], (unsigned long long)(w * fixed + 0.5));
-    }
-  });
+  const bool by_count = q.way == Way::kRank;
+  const double fixed = by_count ? 1.0 : fixed_point(sa.a.V), least = q.least(sa.a.V);
+  if (by_count) {
+    view.row.walk(view.w0, view.w1, [&](float v, int) {
+      const int b = weight.bin(v);
+      if (b < kSliceBins) atomicAdd(&s.mass[b], 1ull);
+    });
+  } else {
+    view.row.walk(view.w0, view.w1, [&](float v, int) {
+      const double w = weight.of(v);
+      x += w;
+      const int b = weight.bin(v);
+      if (w >= least && b < kSliceBins)
+        atomicAdd(&s.mass[b], (unsigned long long)(w * fixed + 0.5));
+    });
+  }
   block_scan<kSliceWaves>(x, s.wave_d, all);
   // Published by agent-scope stores, which write through; every wave waits for
   // its own before the arrival is counted.
-  for (int i = tid; i < kSliceBins; i += kSliceThreads) {
+  for (int i = tid; i < kSliceBins; i += kSliceThreads)
     __hip_atomic_store(sa.mass + rs * kSliceBins + i, s.mass[i], __ATOMIC_RELAXED,
                        __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(sa.count + rs * kSliceBins + i, s.count[i], __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
-  }
   if (tid == 0)
     __hip_atomic_store(reinterpret_cast<unsigned long long*>(sa.total + rs),
                        __builtin_bit_cast(unsigned long long, all), __ATOMIC_RELAXED,
@@ -901,47 +931,43 @@ __global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs
   constexpr int PER = kSliceBins / kSliceThreads;
   const size_t r0 = (size_t)r * sa.S;
   unsigned long long m[PER] = {};
-  uint32_t c[PER] = {};
-#pragma unroll 4
-  for (int i = 0; i < sa.S; i++) {
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-      const size_t at = (r0 + i) * kSliceBins + tid * PER + j;
-      m[j] += __hip_atomic_load(sa.mass + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      c[j] += __hip_atomic_load(sa.count + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+  for (int i = 0; i < kMaxSlices; i++) {
+    if (i >= sa.S) break;
+#pragma unroll
+    for (int j = 0; j < PER; j++)
+      m[j] += __hip_atomic_load(sa.mass + (r0 + i) * kSliceBins + tid * PER + j, __ATOMIC_RELAXED,
+                                __HIP_MEMORY_SCOPE_AGENT);
   }
   all = 0.0;
-  for (int i = 0; i < sa.S; i++)
-    all += __builtin_bit_cast(
-        double, __hip_atomic_load(reinterpret_cast<unsigned long long*>(sa.total + r0 + i),
-                                  __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-  const double unit = 1.0 / fixed, target = (double)q.p * all;
-  double wt = 0.0, unused;
-  uint32_t ct = 0;
 #pragma unroll
-  for (int j = 0; j < PER; j++) {
-    wt += (double)m[j] * unit;
-    ct += c[j];
-  }
-  double before_w = block_scan<kSliceWaves>(wt, s.wave_d, unused) - wt;
-  uint32_t before_c = block_scan_u<kSliceWaves>(ct, s.wave_u) - ct;
+  for (int i = 0; i < kMaxSlices; i++)
+    if (i < sa.S)
+      all += __builtin_bit_cast(
+          double, __hip_atomic_load(reinterpret_cast<unsigned long long*>(sa.total + r0 + i),
+                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  const double unit = 1.0 / fixed, target = by_count ? (double)q.k : (double)q.p * all;
+  double wt = 0.0, unused;
+#pragma unroll
+  for (int j = 0; j < PER; j++) wt += (double)m[j] * unit;
+  const double before = block_scan<kSliceWaves>(wt, s.wave_d, unused) - wt;
   if (tid == 0) s.bin = kSliceBins;
   __syncthreads();
   {
-    double run = before_w;
+    double run = before;
 #pragma unroll
     for (int j = 0; j < PER; j++) {
       run += (double)m[j] * unit;
-      if (c[j] > 0 && run >= target) {
+      if (m[j] > 0 && run >= target) {
         atomicMin(&s.bin, tid * PER + j);
         break;
       }
     }
   }
   __syncthreads();
+  // (no bin: fewer than k tokens have a weight; all bins are before the list)
   int lo = s.bin, hi = s.bin;
-  if (lo < kSliceBins && q.min_p > 0.0) {
+  if (q.min_p > 0.0) {
     // where w = min_p, give or take the bins' rounding
     const double at = -log2(q.min_p) / weight.per * (double)weight.bins * 0.5;
     const int b = at < (double)kSliceBins ? (int)at : kSliceBins;
@@ -952,27 +978,13 @@ __global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs
       lo = max(min(lo, b - 1), 0);
     }
   }
-  // the tokens in them, and what lies before
-  if (tid == 0) s.n = 0;
-  if (tid == lo / PER && lo < kSliceBins) {
-    double w = before_w;
-    uint32_t n = before_c;
-    for (int j = 0; j < PER && tid * PER + j < lo; j++) {
-      w += (double)m[j] * unit;
-      n += c[j];
-    }
-    sa.info[r].below = w;
-    sa.info[r].before = n;
-  }
-  __syncthreads();
-  uint32_t in = 0;
+  if (tid == min(lo / PER, kSliceThreads - 1)) {
+    double w = before;
 #pragma unroll
-  for (int j = 0; j < PER; j++)
-    if (tid * PER + j >= lo && tid * PER + j <= hi) in += c[j];
-  if (in > 0) atomicAdd(&s.n, in);
-  __syncthreads();
-  if (tid == 0) {
-    sa.info[r].lo = lo < kSliceBins && s.n <= (uint32_t)kList ? lo : -1;
+    for (int j = 0; j < PER; j++)
+      if (tid * PER + j < lo) w += (double)m[j] * unit;
+    sa.info[r].below = w;
+    sa.info[r].lo = lo;
     sa.info[r].hi = hi;
     sa.info[r].all = all;
   }
@@ -983,17 +995,15 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SliceArgs 
   __shared__ SliceLds s;
   const int r = blockIdx.y, sl = blockIdx.x, tid = threadIdx.x;
   const RowParams q(sa.a, r);
-  if (q.way != Way::kTopK && q.way != Way::kNucleus) return;
+  if (q.way == Way::kTop || q.way == Way::kTotals || q.way == Way::kWhole) return;
   float top;
   int first;
   row_top(sa, r, top, first);
   if (first < 0) return;
   const SliceInfo info = sa.info[r];
-  if (q.way == Way::kNucleus && info.lo < 0) return;
   const SliceView<E> view(sa, r, sl);
   const size_t rs = (size_t)r * sa.S + sl;
-  const Weight weight = nucleus_weight(q, top, sa.a.V);
-  const double least = q.least(sa.a.V);
+  const Weight weight = slice_weight(q, top, sa.a.V);
   if (tid == 0) s.n = 0;
   __syncthreads();
   auto keep = [&](float v, int i) {
@@ -1005,15 +1015,28 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SliceArgs 
       if (v >= info.cut) keep(v, i);
     });
   } else {
-    view.row.walk(view.w0, view.w1, [&](float v, int i) {
-      const int b = weight.bin(v);
-      if (b >= info.lo && b <= info.hi && weight.of(v) >= least) keep(v, i);
-    });
-    // the slice's weight before the bins
+    // the bins, and the slice's weight before them
     double x = 0.0, below;
-    const double unit = 1.0 / fixed_point(sa.a.V);
-    for (int i = tid; i < info.lo; i += kSliceThreads)
-      x += (double)sa.mass[rs * kSliceBins + i] * unit;
+    if (q.way == Way::kRank) {
+      view.row.walk(view.w0, view.w1, [&](float v, int i) {
+        const int b = weight.bin(v);
+        if (b < info.lo)
+          x += weight.of(v);
+        else if (b <= info.hi && b < kSliceBins)
+          keep(v, i);
+      });
+    } else {
+      view.row.walk(view.w0, view.w1, [&](float v, int i) {
+        const int b = weight.bin(v);
+        if (b >= info.lo && b <= info.hi && b < kSliceBins) keep(v, i);
+      });
+      const double unit = 1.0 / fixed_point(sa.a.V);
+#pragma unroll
+      for (int j = 0; j < kSliceBins / kSliceThreads; j++) {
+        const int i = tid + j * kSliceThreads;
+        if (i < info.lo) x += (double)sa.mass[rs * kSliceBins + i] * unit;
+      }
+    }
     block_scan<kSliceWaves>(x, s.wave_d, below);
     if (tid == 0) sa.total[rs] = below;
   }
@@ -1042,7 +1065,7 @@ __device__ __forceinline__ int join_lists(const SliceArgs& sa, int r, Lds& s) {
   if (i < total) {
     int sl = 0;
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1)
+    for (int d = kMaxSlices / 2; d > 0; d >>= 1)
       if (s.upto[sl + d - 1] <= i) sl += d;
     const uint2 e = sa.list[(r0 + sl) * kList + (i - (sl > 0 ? s.upto[sl - 1] : 0))];
     s.key2[i] = e.x;
@@ -1111,21 +1134,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
   double w_token = 0.0, total = 0.0;
   int n = kList + 1;      // listed tokens
   double all = 0.0;       // the total that top-p is a share of (top-k: the list's)
-  double below = 0.0;     // weight and
-  uint32_t before = 0;    // number of the tokens before the listed
+  double below = 0.0;     // weight (where top-k acts, number) of the tokens before the listed
   bool slices = false;    // the row's weight is in its slices, the list only its last part
   if constexpr (SLICED) {
     if (q.way == Way::kTopK) {
       n = join_lists(sa, r, s);
-    } else if (q.way == Way::kNucleus) {
+    } else if (q.way == Way::kNucleus || q.way == Way::kRank) {
       const SliceInfo info = sa.info[r];
-      if (info.lo >= 0) {
-        n = join_lists(sa, r, s);
-        all = info.all;
-        below = info.below;
-        before = info.before;
-        slices = n <= kList && before > 0;
-      }
+      n = join_lists(sa, r, s);
+      all = info.all;
+      below = info.below;
+      slices = n <= kList && below > 0.0;
     } else if (q.way == Way::kTotals) {
       n = 0;
       slices = true;
@@ -1160,22 +1179,21 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
   }
   if (n <= kList) {
     const int i = threadIdx.x;
-    if (i < n) s.weight[i] = weight.of(value_of_key(s.key[i]));
     if (i == 0) {
       s.found = kList;
       s.lo = 0;
     }
-    __syncthreads();
+    weigh_list(s, n, weight);
     uint32_t rank = 0;
     double above = 0.0, w = 0.0;
     bool in = i < n;
     if (in) {
       rank_of(s, n, i, rank, above);
       w = s.weight[i];
-      if (q.has_k) in = rank < (uint32_t)q.k;
+      if (q.has_k) in = below + (double)rank < (double)q.k;
     }
     if (q.has_k && q.has_p) block_scan(in ? w : 0.0, s.wave_d, all);
-    if (in && q.has_p) in = below + above < (double)q.p * all || rank + before == 0;
+    if (in && q.has_p) in = below + above < (double)q.p * all || (rank == 0 && below == 0.0);
     if (in) in = w >= q.min_p;
     if (!slices) {
       const double upto = block_scan(in ? w : 0.0, s.wave_d, total);
@@ -1230,7 +1248,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
       }
       const int sp = (row.vectors + sa.S - 1) / sa.S;
       const int v0 = min(max(at, 0) * sp, row.vectors), v1 = min(v0 + sp, row.vectors);
-      const Weight bins = nucleus_weight(q, weight.top, a.V);
+      const Weight bins = slice_weight(q, weight.top, a.V);
       const int lo = totals ? 0 : sa.info[r].lo;
       const Found f = find_within(row, v0, v1, base, target, s, [&](float v, int idx) {
         const double y = weight.of(v);
@@ -1268,7 +1286,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
 
 struct Layout {
   int S = 1;  // 1: no slices
-  size_t thread_top = 0, first = 0, total = 0, mass = 0, count = 0, listed = 0, list = 0, info = 0,
+  size_t thread_top = 0, first = 0, total = 0, mass = 0, listed = 0, list = 0, info = 0,
          arrived = 0, bytes = 0;
 };
 
@@ -1292,7 +1310,6 @@ Layout layout_of(int rows, int V) {
   l.thread_top = put(n * 4 * kSliceThreads);
   l.total = put(n * 8);
   l.mass = put(n * 8 * kSliceBins);
-  l.count = put(n * 4 * kSliceBins);
   l.listed = put(n * 4);
   l.list = put(n * 8 * kList);
   l.info = put((size_t)rows * sizeof(SliceInfo));
@@ -1359,7 +1376,6 @@ int sde_sample(const void* d_logits, int64_t row_stride, int dtype, int n_rows, 
     sa.thread_top = reinterpret_cast<float*>(w + l.thread_top);
     sa.total = reinterpret_cast<double*>(w + l.total);
     sa.mass = reinterpret_cast<unsigned long long*>(w + l.mass);
-    sa.count = reinterpret_cast<uint32_t*>(w + l.count);
     sa.listed = reinterpret_cast<uint32_t*>(w + l.listed);
     sa.list = reinterpret_cast<uint2*>(w + l.list);
     sa.info = reinterpret_cast<SliceInfo*>(w + l.info);

@@ -76,45 +76,95 @@ __device__ __forceinline__ float value_of_key(uint32_t k) {
   return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
-// 2^t for t <= 0, to 1e-14 of it, and 0 from -1100 down: the integer part to the
-// exponent, the rest f in [-1/2, 1/2] by the series of exp(f ln 2).
-__device__ __forceinline__ double exp2_f64(double t) {
-  t = fmax(t, -1100.0);
-  const double n = rint(t);
-  const double f = t - n;
-  double y = 4.44553827187081e-10;  // ln(2)^11 / 11!
-  y = fma(y, f, 7.054911620801121e-09);
-  y = fma(y, f, 1.0178086009239696e-07);
-  y = fma(y, f, 1.3215486790144305e-06);
-  y = fma(y, f, 1.5252733804059838e-05);
-  y = fma(y, f, 0.00015403530393381606);
-  y = fma(y, f, 0.0013333558146428441);
-  y = fma(y, f, 0.009618129107628477);
-  y = fma(y, f, 0.055504108664821576);
-  y = fma(y, f, 0.2402265069591007);
-  y = fma(y, f, 0.6931471805599453);
-  y = fma(y, f, 1.0);
-  return ldexp(y, (int)n);
+constexpr int kPowers = 256;
+
+// 2^(i / 256), i < 256, by the series of exp(f ln 2): to 1e-14 (f < 1: the
+// twelfth term is 2.5e-11 of it; f is halved and the result squared).
+template <int THREADS>
+__device__ __forceinline__ void fill_powers(double* power) {
+  for (int i = threadIdx.x; i < kPowers; i += THREADS) {
+    const double f = (double)i * (0.5 / kPowers);
+    double y = 4.44553827187081e-10;  // ln(2)^11 / 11!
+    y = fma(y, f, 7.054911620801121e-09);
+    y = fma(y, f, 1.0178086009239696e-07);
+    y = fma(y, f, 1.3215486790144305e-06);
+    y = fma(y, f, 1.5252733804059838e-05);
+    y = fma(y, f, 0.00015403530393381606);
+    y = fma(y, f, 0.0013333558146428441);
+    y = fma(y, f, 0.009618129107628477);
+    y = fma(y, f, 0.055504108664821576);
+    y = fma(y, f, 0.2402265069591007);
+    y = fma(y, f, 0.6931471805599453);
+    y = fma(y, f, 1.0);
+  power[i] = y * y;
+  }
 }
 
-// A row's weights: 1 at the max (also an infinite one), 0 at -inf.
+// A row's weights: 1 at the max (also an infinite one), 0 at -inf and below
+// 2^-1000.  2^t to 2e-13 of it: t to 1/256ths, whose powers lie in LDS, and a
+// cubic for the rest, f in [-1/512, 1/512]: ten 64-bit operations, where a series
+// alone takes seventeen.
 struct Weight {
-  float top;      // the row's max
-  double per;     // log2(e) / T
-  float bins;     // histogram bins per unit of (max - x) / 2
-  int limit;      // and their number
-  __device__ __forceinline__ double of(float x) const {
-    // (NaN where an infinite T meets -inf: 0, as its -1100)
-    const double w = exp2_f64(((double)x - (double)top) * per);
+  float top;            // the row's max
+  float least;          // weights from here down are 0
+  double per;           // 256 log2(e) / T
+  uint32_t bin_mul;     // histogram bins per 1/256 of a factor 2, 16 bits of fraction
+  uint32_t bin_end;     // 1/256ths that reach the last bin
+  int limit;            // number of bins
+  const double* power;  // fill_powers'
+  __device__ __forceinline__ Weight(float max_x, float T, const double* powers)
+      : top(max_x), power(powers) {
+    per = 1.4426950408889634 * kPowers / (double)T;
+    least = top - (1000.f * kPowers) / (float)per;
+  }
+  // `n` bins of 1 / per_log2 of a factor 2
+  __device__ __forceinline__ void set_bins(float per_log2, int n) {
+    bin_mul = (uint32_t)fmaxf(per_log2 * (65536.f / kPowers), 1.f);
+    bin_end = (uint32_t)(((uint64_t)n << 16) / bin_mul) + 1;
+    limit = n;
+  }
+  // The weight, and `n`: its log2 to 1/256ths (meaningless where it is 0).
+  // NaN weighs 0.
+  __device__ __forceinline__ double of(float x, int& n) const {
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is rint(t)
+    const double t = ((double)x - (double)top) * per;
+    const double shifted = t + kRound;
+    const double f = t - (shifted - kRound);
+    n = (int)(uint32_t)__builtin_bit_cast(uint64_t, shifted);
+    double y = fma(f, 3.308302680541371e-09, 3.665565596910106e-06);
+    y = fma(f, y, 0.0027076061740622863);
+    y = fma(f, y, 1.0) * power[n & (kPowers - 1)];
+    // (above 2^-1000: the exponent takes the sum)
+    uint64_t bits = __builtin_bit_cast(uint64_t, y);
+    bits += (uint64_t)(uint32_t)((n >> 8) << 20) << 32;
+    const double w = x > least ? __builtin_bit_cast(double, bits) : 0.0;
+    n = x == top ? 0 : n;
     return x == top ? 1.0 : w;
   }
-  // 0 at the max, rising as x falls; `limit`: left out
+  __device__ __forceinline__ double of(float x) const {
+    int n;
+    return of(x, n);
+  }
+  // 0 at the max, rising as x falls, of a weight that is not 0; `limit` and
+  // beyond: left out
+  __device__ __forceinline__ int bin_of(int n) const {
+    return (int)((min((uint32_t)-n, bin_end) * (uint64_t)bin_mul) >> 16);
+  }
+  // `limit` also for weights of 0
   __device__ __forceinline__ int bin(float x) const {
-    if (x == top) return 0;
-    if (x == -INFINITY) return limit;
-    return (int)fminf((0.5f * top - 0.5f * x) * bins, (float)limit);  // (halves: no overflow)
+    int n;
+    return of(x, n) > 0.0 ? min(bin_of(n), limit) : limit;
   }
 };
+
+// Fixed point of the histograms' weights: V of them fit 63 bits, one fits 52.
+__device__ __forceinline__ double fixed_point(int V) { return ldexp(1.0, min(30 + __clz(V), 51)); }
+// w * fixed, rounded (the sum's low bits).
+__device__ __forceinline__ unsigned long long to_fixed(double w, double fixed) {
+  constexpr double k2p52 = 4503599627370496.0;
+  return __builtin_bit_cast(unsigned long long, fma(w, fixed, k2p52)) -
+         __builtin_bit_cast(unsigned long long, k2p52);
+}
 
 // What is kept: keys above `key`, and the key itself up to index `last`.
 struct Kept {
@@ -138,54 +188,83 @@ struct RowView {
     shift = (int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
     vectors = (V + shift + VEC - 1) / VEC;
   }
-  // Elements of vector v (none from `end` on); places outside the row and NaN
-  // read as -inf.
-  __device__ __forceinline__ void load(int v, int end, T (&e)[VEC]) const {
+  // Vector v (nothing from `end` on); places outside the row read as -inf.
+  __device__ __forceinline__ uint4 load(int v, int end) const {
     const int i0 = v * VEC - shift;
+    uint4 raw;
     if (v < end && i0 >= 0 && i0 + VEC <= V) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(p + i0);
-      __builtin_memcpy(e, &raw, 16);
+      raw = *reinterpret_cast<const uint4*>(p + i0);
     } else {
+      T e[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; k++)
         e[k] = v < end && i0 + k >= 0 && i0 + k < V ? p[i0 + k] : E::put(-INFINITY);
+      __builtin_memcpy(&raw, e, 16);
+    }
+    return raw;
+  }
+  // (NaN passes no compare and weighs nothing)
+  static __device__ __forceinline__ float value(T e) { return E::get(e); }
+  // f(value, index) over a vector's elements, in pairs: the loop is rolled, since
+  // an exponential's code a dozen times over costs more to fetch than to run.
+  template <class F>
+  static __device__ __forceinline__ void each(uint4 c, int index, F f) {
+#pragma unroll 1
+    for (int i = 0; i < VEC; i += 2) {
+      if constexpr (sizeof(T) == 4) {
+        f(value(__builtin_bit_cast(float, c.x)), index + i);
+        f(value(__builtin_bit_cast(float, c.y)), index + i + 1);
+        c.x = c.z;
+        c.y = c.w;
+      } else {
+        f(value((T)(c.x & 0xFFFFu)), index + i);
+        f(value((T)(c.x >> 16)), index + i + 1);
+        c.x = c.y;
+        c.y = c.z;
+        c.z = c.w;
+      }
     }
   }
-  static __device__ __forceinline__ float value(T e) {
-    const float x = E::get(e);
-    return x == x ? x : -INFINITY;
-  }
   // f(value, index) over vectors [v0, v1), the wave's lanes side by side; a
-  // lane's indexes rise.
-  template <class F>
+  // lane's indexes rise.  LIGHT: a few instructions, unrolled.
+  template <bool LIGHT = false, class F>
   __device__ __forceinline__ void walk(int v0, int v1, F f) const {
-    constexpr int U = 16 / VEC;  // vectors in flight
+    constexpr int U = 4;  // vectors in flight
     const int lane = threadIdx.x & 63;
 #pragma unroll 1
     for (int v = v0; v < v1; v += 64 * U) {
-      T e[U][VEC];
+      uint4 raw[U];
       if (v + 64 * U <= v1 && v * VEC >= shift && (v + 64 * U) * VEC - shift <= V) {
 #pragma unroll
-        for (int k = 0; k < U; k++) {
-          const uint4 raw =
-              *reinterpret_cast<const uint4*>(p + ((v + 64 * k + lane) * VEC - shift));
-          __builtin_memcpy(e[k], &raw, 16);
-        }
+        for (int k = 0; k < U; k++)
+          raw[k] = *reinterpret_cast<const uint4*>(p + ((v + 64 * k + lane) * VEC - shift));
       } else {
 #pragma unroll
-        for (int k = 0; k < U; k++) load(v + 64 * k + lane, v1, e[k]);
+        for (int k = 0; k < U; k++) raw[k] = load(v + 64 * k + lane, v1);
       }
+      if constexpr (LIGHT) {
 #pragma unroll
-      for (int k = 0; k < U; k++) {
+        for (int k = 0; k < U; k++) {
+          T e[VEC];
+          __builtin_memcpy(e, &raw[k], 16);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) f(value(e[k][i]), (v + 64 * k + lane) * VEC - shift + i);
+          for (int i = 0; i < VEC; i++) f(value(e[i]), (v + 64 * k + lane) * VEC - shift + i);
+        }
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < U; k++) {
+          each(raw[0], (v + 64 * k + lane) * VEC - shift, f);
+#pragma unroll
+          for (int j = 0; j + 1 < U; j++) raw[j] = raw[j + 1];
+        }
       }
     }
   }
 };
 
 struct Lds {
-  uint32_t count[kBins];
+  double power[kPowers];
+  __attribute__((aligned(16))) uint32_t count[kBins];
   unsigned long long mass[kBins];
   __attribute__((aligned(16))) uint32_t key[kList];
   int index[kList];
@@ -337,18 +416,14 @@ __device__ __forceinline__ Found find_within(const RowView<E>& row, int v0, int 
   int tail = -1;
   double tail_f = 0.0;
   for (int v = a; v < b; v++) {
-    typename E::type e[RowView<E>::VEC];
-    row.load(v, v1, e);
-#pragma unroll
-    for (int i = 0; i < RowView<E>::VEC; i++) {
-      const int idx = v * RowView<E>::VEC - row.shift + i;
-      const double y = f(row.value(e[i]), idx);
+    row.each(row.load(v, v1), v * RowView<E>::VEC - row.shift, [&](float x, int idx) {
+      const double y = f(x, idx);
       mine += y;
       if (y > 0.0) {
         tail = idx;
         tail_f = y;
       }
-    }
+    });
   }
   double unused;
   const double upto = base + block_scan(mine, s.wave_d, unused);
@@ -361,18 +436,14 @@ __device__ __forceinline__ Found find_within(const RowView<E>& row, int v0, int 
     if ((int)threadIdx.x == at) {
       double sum = upto - mine;
       for (int v = a; v < b; v++) {
-        typename E::type e[RowView<E>::VEC];
-        row.load(v, v1, e);
-#pragma unroll
-        for (int i = 0; i < RowView<E>::VEC; i++) {
-          const int idx = v * RowView<E>::VEC - row.shift + i;
-          const double y = f(row.value(e[i]), idx);
+        row.each(row.load(v, v1), v * RowView<E>::VEC - row.shift, [&](float x, int idx) {
+          const double y = f(x, idx);
           sum += y;
           if (y > 0.0 && sum > target && s.out_i[0] < 0) {
             s.out_i[0] = idx;
             s.out_d[0] = y;
           }
-        }
+        });
       }
       if (s.out_i[0] < 0) {
         s.out_i[0] = tail;
@@ -460,16 +531,17 @@ __device__ __forceinline__ void sort_list(Lds& s, int n) {
   __syncthreads();
 }
 
-// Gathers the tokens for which `in` holds into s.key / s.index in index order;
+// Gathers the tokens for which `in` holds into s.key2 / s.index2, in no order;
 // their number, or kList + 1 for more than fit.
-template <class E, class P>
-__device__ __forceinline__ int gather(const RowView<E>& row, Lds& s, P in) {
+template <bool LIGHT, class E, class P>
+__device__ __forceinline__ int collect(const RowView<E>& row, Lds& s, P in) {
   const int wave = threadIdx.x >> 6;
   const int per = (row.vectors + kWaves - 1) / kWaves;
   __syncthreads();
   if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
-  row.walk(min(wave * per, row.vectors), min((wave + 1) * per, row.vectors), [&](float v, int i) {
+  row.template walk<LIGHT>(min(wave * per, row.vectors), min((wave + 1) * per, row.vectors),
+                           [&](float v, int i) {
     if (in(v, i)) {
       const uint32_t n = atomicAdd(&s.n, 1u);
       if (n < kList) {
@@ -479,10 +551,15 @@ __device__ __forceinline__ int gather(const RowView<E>& row, Lds& s, P in) {
     }
   });
   __syncthreads();
-  const uint32_t n = s.n;
-  if (n > kList) return kList + 1;
-  sort_list(s, (int)n);
-  return (int)n;
+  return (int)min(s.n, (uint32_t)kList + 1);
+}
+
+// The same into s.key / s.index in index order.
+template <class E, class P>
+__device__ __forceinline__ int gather(const RowView<E>& row, Lds& s, P in) {
+  const int n = collect<false>(row, s, in);
+  if (n <= kList) sort_list(s, n);
+  return n;
 }
 
 // The listed tokens' weights to s.weight, and the list filled up to a multiple
@@ -521,10 +598,11 @@ __device__ __forceinline__ void rank_of(const Lds& s, int n, int i, uint32_t& ra
 
 // Narrows the last kept token down to a key and an index, over the tokens of
 // `kept`: the k-th of them (BY_COUNT), or the one whose weight, with all before
-// it, reaches `m`.
+// it, reaches `m`.  `ready`: the first histogram is there.
 template <bool BY_COUNT, class E>
 __device__ __forceinline__ Kept last_kept(const RowView<E>& row, const Weight& weight, Kept kept,
-                                          uint32_t k, double m, double fixed, Lds& s) {
+                                          uint32_t k, double m, double fixed, Lds& s,
+                                          bool ready = false) {
   const int wave = threadIdx.x >> 6;
   const int per = (row.vectors + kWaves - 1) / kWaves;
   const int w0 = min(wave * per, row.vectors), w1 = min((wave + 1) * per, row.vectors);
@@ -539,15 +617,18 @@ __device__ __forceinline__ Kept last_kept(const RowView<E>& row, const Weight& w
     return key < lo || key > hi ? kBins : (int)((hi - key) / width);
   };
   for (;;) {
-    clear_histogram(s);
-    row.walk(w0, w1, [&](float v, int i) {
-      const int b = bin_of(v);
-      if (b < kBins && weight.bin(v) < kBins && kept.has(key_of(v), i)) {
-        atomicAdd(&s.count[b], 1u);
-        atomicAdd(&s.mass[b], (unsigned long long)(weight.of(v) * fixed + 0.5));
-      }
-    });
-    __syncthreads();
+    if (!ready) {
+      clear_histogram(s);
+      row.walk(w0, w1, [&](float v, int i) {
+        const int b = bin_of(v);
+        if (b < kBins && weight.bin(v) < kBins && kept.has(key_of(v), i)) {
+          atomicAdd(&s.count[b], 1u);
+          atomicAdd(&s.mass[b], to_fixed(weight.of(v), fixed));
+        }
+      });
+      __syncthreads();
+    }
+    ready = false;
     const BinAt at = find_bin<BY_COUNT>(s, k - before, m - mass, 1.0 / fixed, width > 0);
     if (at.bin == kBins) return kept;  // everything there is
     before += at.before;
@@ -627,20 +708,19 @@ __device__ __forceinline__ Kept last_kept(const RowView<E>& row, const Weight& w
 // One workgroup walks a row of 128256 at some 20 us a time where weights are
 // needed.  With fewer rows than fill the chip, a row is cut into slices of
 // vectors, a workgroup each, in three launches before the row's own:
-//  max      the slice's max, and each thread's for top-k;
-//  weights  top-k up to kList: the cut, a bound of the k-th largest (one
-//           workgroup a row);
-//           a larger k, or top-p: the slice's histogram, of tokens or of weight,
-//           and its total; the last workgroup of a row joins them and finds the
-//           bin that holds the last kept token;
-//           neither: the slice's total;
-//  gather   the tokens at or above the cut, or in that bin, into a list per
-//           slice, and the slice's weight before the bin.
+//  max      the slice's max;
+//  weights  top-k above kList, or top-p: the slice's histogram, of tokens or of
+//           weight, and its total; the last workgroup of a row joins them and
+//           finds the bin that holds the last kept token;
+//           no filter, or min-p alone: the slice's total;
+//  gather   the tokens in that bin into a list per slice, and the slice's weight
+//           before it.
 // The row's workgroup then has the lists to compare, and the slices' weights
 // to find the one that holds the token, which alone it walks.
-// Which way a row goes is told by its parameters; one whose list would be too
-// long (flat rows, ties), or with both a large k and top-p, is walked whole by
-// its workgroup.
+// Which way a row goes is told by its parameters.  Rows with k up to kList leave
+// the slices alone (two light walks: 128256 fp32 values 24 us in one workgroup,
+// 34 with a cut and lists from 16 slices), and one whose list would be too long (flat rows, ties), or with
+// both a large k and top-p, is walked whole by its workgroup.
 
 enum class Way { kTop, kTopK, kRank, kNucleus, kTotals, kWhole };
 
@@ -651,11 +731,15 @@ struct RowParams {
   bool has_k, has_p;
   Way way;
   __device__ __forceinline__ RowParams(const SampleArgs& a, int r) {
-    T = a.temperature ? a.temperature[r] : 1.f;
-    u = a.u[r];
-    k = a.top_k ? a.top_k[r] : 0;
-    p = a.top_p ? a.top_p[r] : 1.f;
-    min_p = a.min_p && a.min_p[r] > 0.f ? fmin((double)a.min_p[r], 1.0) : 0.0;
+    // (all five loads at once: a branch round each would wait for each)
+    const float tv = (a.temperature ? a.temperature : a.u)[r], uv = a.u[r];
+    const int32_t kv = (a.top_k ? a.top_k : reinterpret_cast<const int32_t*>(a.u))[r];
+    const float pv = (a.top_p ? a.top_p : a.u)[r], mv = (a.min_p ? a.min_p : a.u)[r];
+    T = a.temperature ? tv : 1.f;
+    u = uv;
+    k = a.top_k ? kv : 0;
+    p = a.top_p ? pv : 1.f;
+    min_p = a.min_p && mv > 0.f ? fmin((double)mv, 1.0) : 0.0;
     has_k = k > 0 && k < a.V;
     has_p = p < 1.f;
     if (!(T >= kMinTemperature))
@@ -672,12 +756,9 @@ struct RowParams {
   }
 };
 
-// Fixed point of the histograms' weights: V of them fit 63 bits.
-__device__ __forceinline__ double fixed_point(int V) { return ldexp(1.0, 30 + __clz(V)); }
-
 struct SliceInfo {  // of a row
-  float cut;        // top-k: the lowest value listed
-  int lo, hi;       // the bins listed
+  float low, high;  // the values listed
+  int lo;           // their first bin
   double below;     // what lies before them: weight (tokens, where top-k acts)
   double all;       // the row's weight
 };
@@ -687,7 +768,6 @@ struct SliceArgs {
   int S;                      // slices of a row
   float* top;                 // [rows][S]
   int* first;                 // [rows][S]
-  float* thread_top;          // [rows][S][kSliceThreads]
   double* total;              // [rows][S]; after the gather: the weight before bin lo
   unsigned long long* mass;   // [rows][S][kSliceBins] (tokens, where top-k acts)
   uint32_t* listed;           // [rows][S]
@@ -697,7 +777,8 @@ struct SliceArgs {
 };
 
 struct SliceLds {
-  unsigned long long mass[kSliceBins];
+  double power[kPowers];
+  __attribute__((aligned(16))) unsigned long long mass[kSliceBins];
   double wave_d[kSliceWaves];
   uint32_t wave_u[kSliceWaves];
   float wave_f[kSliceWaves];
@@ -751,14 +832,12 @@ __device__ __forceinline__ void row_top(const SliceArgs& sa, int r, float& x, in
 
 // The bins of a nucleus: from the max down to the least weight that can be its
 // last.  Of a larger k's: 2^-64 of the max, below which nothing is drawn.
-__device__ __forceinline__ Weight slice_weight(const RowParams& q, float top, int V) {
-  Weight w;
-  w.top = top;
-  w.per = 1.4426950408889634 / (double)q.T;
+__device__ __forceinline__ Weight slice_weight(const RowParams& q, float top, int V,
+                                               const double* power) {
+  Weight w(top, q.T, power);
   const float range =
       q.way == Way::kNucleus ? log2f((float)V / (1.f - fmaxf(q.p, 0.f))) + 2.f : 64.f;
-  w.bins = 2.f * (float)w.per * ((float)kSliceBins / range);
-  w.limit = kSliceBins;
+  w.set_bins((float)kSliceBins / range, kSliceBins);
   return w;
 }
 
@@ -766,17 +845,17 @@ template <class E>
 __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SliceArgs sa) {
   __shared__ SliceLds s;
   const int r = blockIdx.y, sl = blockIdx.x, tid = threadIdx.x;
+  if (RowParams(sa.a, r).way == Way::kTopK) return;
   const SliceView<E> view(sa, r, sl);
   float x = -INFINITY;
   int i = -1;
-  view.row.walk(view.w0, view.w1, [&](float v, int at) {
+  view.row.template walk<true>(view.w0, view.w1, [&](float v, int at) {
     if (v > x) {
       x = v;
       i = at;
     }
   });
   const size_t rs = (size_t)r * sa.S + sl;
-  if (RowParams(sa.a, r).way == Way::kTopK) sa.thread_top[rs * kSliceThreads + tid] = x;
   wave_top(x, i);
   if ((tid & 63) == 0) {
     s.wave_f[tid >> 6] = x;
@@ -796,71 +875,18 @@ __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SliceArgs sa)
   }
 }
 
-// The lowest of the threads' maxima that at least k of them reach (to a bin's
-// width): at least k tokens do.
-__device__ __forceinline__ float top_k_cut(const SliceArgs& sa, int r, int k, float top,
-                                           SliceLds& s) {
-  const int tid = threadIdx.x;
-  const float* t = sa.thread_top + (size_t)r * sa.S * kSliceThreads + tid;
-  float x[kMaxSlices];
-#pragma unroll
-  for (int i = 0; i < kMaxSlices; i++)
-    x[i] = i < sa.S ? t[(size_t)i * kSliceThreads] : -INFINITY;
-  uint32_t* const count = reinterpret_cast<uint32_t*>(s.mass);
-  for (int i = tid; i < kSliceBins; i += kSliceThreads) count[i] = 0;
-  if (tid == 0) {
-    s.key = 0xFFFFFFFFu;
-    s.bin = kSliceBins;
-    s.n = 0;
+// The lowest key (of a finite value) in bins up to b; the max's is in bin 0.
+__device__ __forceinline__ uint32_t lowest_key(const Weight& weight, int b) {
+  uint32_t lo = key_of(-FLT_MAX), hi = key_of(weight.top);
+#pragma unroll 1
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (weight.bin(value_of_key(mid)) <= b)
+      hi = mid;
+    else
+      lo = mid + 1;
   }
-  __syncthreads();
-  float low = INFINITY;
-  uint32_t live = 0;
-#pragma unroll
-  for (int i = 0; i < kMaxSlices; i++)
-    if (x[i] > -INFINITY) {
-      low = fminf(low, x[i]);
-      live++;
-    }
-  if (live > 0) {
-    atomicMin(&s.key, key_of(low));
-    atomicAdd(&s.n, live);
-  }
-  __syncthreads();
-  if (s.n < (uint32_t)k) return -FLT_MAX;  // every token with a weight
-  low = value_of_key(s.key);
-  const float span = 0.5f * top - 0.5f * low;
-  const float scale = span > 0.f && span < INFINITY ? (float)(kSliceBins - 1) / span : 0.f;
-  auto bin = [&](float v) {
-    return v == top ? 0 : (int)fminf((0.5f * top - 0.5f * v) * scale, (float)(kSliceBins - 1));
-  };
-#pragma unroll
-  for (int i = 0; i < kMaxSlices; i++)
-    if (x[i] > -INFINITY) atomicAdd(&count[bin(x[i])], 1u);
-  __syncthreads();
-  constexpr int PER = kSliceBins / kSliceThreads;
-  uint32_t c = 0;
-#pragma unroll
-  for (int i = 0; i < PER; i++) c += count[tid * PER + i];
-  uint32_t run = block_scan_u<kSliceWaves>(c, s.wave_u) - c;
-#pragma unroll
-  for (int i = 0; i < PER; i++) {
-    run += count[tid * PER + i];
-    if (run >= (uint32_t)k) {
-      atomicMin(&s.bin, tid * PER + i);
-      break;
-    }
-  }
-  if (tid == 0) s.key = 0xFFFFFFFFu;
-  __syncthreads();
-  const int b = s.bin;
-  low = INFINITY;
-#pragma unroll
-  for (int i = 0; i < kMaxSlices; i++)
-    if (x[i] > -INFINITY && bin(x[i]) <= b) low = fminf(low, x[i]);
-  if (low < INFINITY) atomicMin(&s.key, key_of(low));
-  __syncthreads();
-  return s.key == 0xFFFFFFFFu ? top : value_of_key(s.key);
+  return lo;
 }
 
 template <class E>
@@ -868,19 +894,16 @@ __global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs
   __shared__ SliceLds s;
   const int r = blockIdx.y, sl = blockIdx.x, tid = threadIdx.x;
   const RowParams q(sa.a, r);
-  if (q.way == Way::kTop || q.way == Way::kWhole || (q.way == Way::kTopK && sl > 0)) return;
+  if (q.way == Way::kTop || q.way == Way::kWhole || q.way == Way::kTopK) return;
   float top;
   int first;
   row_top(sa, r, top, first);
   if (first < 0) return;
-  if (q.way == Way::kTopK) {
-    const float cut = top_k_cut(sa, r, q.k, top, s);
-    if (tid == 0) sa.info[r].cut = cut;
-    return;
-  }
+  fill_powers<kSliceThreads>(s.power);
   const SliceView<E> view(sa, r, sl);
   const size_t rs = (size_t)r * sa.S + sl;
-  const Weight weight = slice_weight(q, top, sa.a.V);
+  const Weight weight = slice_weight(q, top, sa.a.V, s.power);
+  __syncthreads();
   double x = 0.0, all;
   if (q.way == Way::kTotals) {
     view.row.walk(view.w0, view.w1, [&](float v, int) {
@@ -902,11 +925,11 @@ __global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs
     });
   } else {
     view.row.walk(view.w0, view.w1, [&](float v, int) {
-      const double w = weight.of(v);
+      int n;
+      const double w = weight.of(v, n);
       x += w;
-      const int b = weight.bin(v);
-      if (w >= least && b < kSliceBins)
-        atomicAdd(&s.mass[b], (unsigned long long)(w * fixed + 0.5));
+      const int b = weight.bin_of(n);
+      if (w >= least && b < kSliceBins) atomicAdd(&s.mass[b], to_fixed(w, fixed));
     });
   }
   block_scan<kSliceWaves>(x, s.wave_d, all);
@@ -969,7 +992,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs
   int lo = s.bin, hi = s.bin;
   if (q.min_p > 0.0) {
     // where w = min_p, give or take the bins' rounding
-    const double at = -log2(q.min_p) / weight.per * (double)weight.bins * 0.5;
+    const double at = -log2(q.min_p) * kPowers * (double)weight.bin_mul * (1.0 / 65536.0);
     const int b = at < (double)kSliceBins ? (int)at : kSliceBins;
     if (b + 1 < lo) {
       lo = max(b - 1, 0);
@@ -985,9 +1008,14 @@ __global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs
       if (tid * PER + j < lo) w += (double)m[j] * unit;
     sa.info[r].below = w;
     sa.info[r].lo = lo;
-    sa.info[r].hi = hi;
     sa.info[r].all = all;
   }
+  // The values in those bins (bins rise as values fall), by bisection: two
+  // compares tell in what follows.
+  if (tid == 0) sa.info[r].low = value_of_key(lowest_key(weight, min(hi, kSliceBins - 1)));
+  if (tid == 64)
+    sa.info[r].high =
+        lo == 0 ? INFINITY : value_of_key(lowest_key(weight, min(lo, kSliceBins) - 1) - 1);
 }
 
 template <class E>
@@ -995,7 +1023,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SliceArgs 
   __shared__ SliceLds s;
   const int r = blockIdx.y, sl = blockIdx.x, tid = threadIdx.x;
   const RowParams q(sa.a, r);
-  if (q.way == Way::kTop || q.way == Way::kTotals || q.way == Way::kWhole) return;
+  if (q.way != Way::kRank && q.way != Way::kNucleus) return;
   float top;
   int first;
   row_top(sa, r, top, first);
@@ -1003,49 +1031,39 @@ __global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SliceArgs 
   const SliceInfo info = sa.info[r];
   const SliceView<E> view(sa, r, sl);
   const size_t rs = (size_t)r * sa.S + sl;
-  const Weight weight = slice_weight(q, top, sa.a.V);
+  const Weight weight = slice_weight(q, top, sa.a.V, s.power);
+  if (q.way == Way::kRank) fill_powers<kSliceThreads>(s.power);
   if (tid == 0) s.n = 0;
   __syncthreads();
   auto keep = [&](float v, int i) {
     const uint32_t n = atomicAdd(&s.n, 1u);
     if (n < kList) sa.list[rs * kList + n] = make_uint2(key_of(v), (uint32_t)i);
   };
-  if (q.way == Way::kTopK) {
-    view.row.walk(view.w0, view.w1, [&](float v, int i) {
-      if (v >= info.cut) keep(v, i);
+  view.row.template walk<true>(view.w0, view.w1, [&](float v, int i) {
+    if (v >= info.low && v <= info.high) keep(v, i);
+  });
+  // the slice's weight before the listed values
+  double x = 0.0, below;
+  if (q.way == Way::kRank) {
+    view.row.walk(view.w0, view.w1, [&](float v, int) {
+      if (v > info.high) x += weight.of(v);
     });
   } else {
-    // the bins, and the slice's weight before them
-    double x = 0.0, below;
-    if (q.way == Way::kRank) {
-      view.row.walk(view.w0, view.w1, [&](float v, int i) {
-        const int b = weight.bin(v);
-        if (b < info.lo)
-          x += weight.of(v);
-        else if (b <= info.hi && b < kSliceBins)
-          keep(v, i);
-      });
-    } else {
-      view.row.walk(view.w0, view.w1, [&](float v, int i) {
-        const int b = weight.bin(v);
-        if (b >= info.lo && b <= info.hi && b < kSliceBins) keep(v, i);
-      });
-      const double unit = 1.0 / fixed_point(sa.a.V);
+    const double unit = 1.0 / fixed_point(sa.a.V);
 #pragma unroll
-      for (int j = 0; j < kSliceBins / kSliceThreads; j++) {
-        const int i = tid + j * kSliceThreads;
-        if (i < info.lo) x += (double)sa.mass[rs * kSliceBins + i] * unit;
-      }
+    for (int j = 0; j < kSliceBins / kSliceThreads; j++) {
+      const int i = tid + j * kSliceThreads;
+      if (i < info.lo) x += (double)sa.mass[rs * kSliceBins + i] * unit;
     }
-    block_scan<kSliceWaves>(x, s.wave_d, below);
-    if (tid == 0) sa.total[rs] = below;
   }
+  block_scan<kSliceWaves>(x, s.wave_d, below);
+  if (tid == 0) sa.total[rs] = below;
   __syncthreads();
   if (tid == 0) sa.listed[rs] = s.n;
 }
 
-// The row's lists into s.key / s.index in index order; their number, or kList + 1
-// for more than fit.  s.upto[i]: tokens of slices 0 .. i.
+// The row's lists into s.key2 / s.index2; their number, or kList + 1 for more than
+// fit.  s.upto[i]: tokens of slices 0 .. i.
 __device__ __forceinline__ int join_lists(const SliceArgs& sa, int r, Lds& s) {
   const int lane = threadIdx.x & 63;
   const size_t r0 = (size_t)r * sa.S;
@@ -1072,8 +1090,100 @@ __device__ __forceinline__ int join_lists(const SliceArgs& sa, int r, Lds& s) {
     s.index2[i] = (int)e.y;
   }
   __syncthreads();
-  sort_list(s, (int)total);
   return (int)total;
+}
+
+// The token of a row whose whole kept weight is among n <= 64 listed tokens, by
+// one wave without a barrier: s.key2 / s.index2 in any order.
+__device__ __forceinline__ void finish_few(const SampleArgs& a, int r, const RowParams& q,
+                                           const Weight& weight, int n, double all, Lds& s) {
+  const int i = threadIdx.x;
+  {
+    const int me = i < n ? s.index2[i] : INT32_MAX;
+    int at = 0;
+    for (int j = 0; j < n; j++) at += __builtin_amdgcn_readlane(me, j) < me ? 1 : 0;
+    if (i < n) {
+      s.key[at] = s.key2[i];
+      s.index[at] = me;
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const uint32_t key = i < n ? s.key[i] : 0;
+  double w = i < n ? weight.of(value_of_key(key)) : 0.0;
+  const uint64_t wb = __builtin_bit_cast(uint64_t, w);
+  uint32_t rank = 0;
+  double above = 0.0;
+  for (int j = 0; j < n; j++) {
+    const uint32_t o = __builtin_amdgcn_readlane(key, j);
+    const uint64_t b = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)wb, j) |
+                       ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(wb >> 32), j)
+                        << 32);
+    const bool first = o > key || (o == key && j < i);
+    rank += first ? 1u : 0u;
+    above += first ? __builtin_bit_cast(double, b) : 0.0;
+  }
+  bool in = i < n && (!q.has_k || rank < (uint32_t)q.k);
+  if (q.has_k && q.has_p) {
+    all = in ? w : 0.0;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
+  }
+  if (in && q.has_p) in = above < (double)q.p * all || rank == 0;
+  if (in) in = w >= q.min_p && w > 0.0;
+  double upto = in ? w : 0.0;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double y = __shfl_up(upto, d, 64);
+    if (i >= d) upto += y;
+  }
+  const double total = __shfl(upto, 63, 64);
+  const uint64_t passed = __builtin_amdgcn_ballot_w64(in && upto > q.u * total);
+  const uint64_t live = __builtin_amdgcn_ballot_w64(in);
+  // (u at or above 1, or rounding: the last kept)
+  const int at = passed ? __builtin_ctzll(passed) : 63 - __builtin_clzll(live);
+  if (i == at) {
+    a.tokens[r] = s.index[i];
+    if (a.probs) a.probs[r] = (float)(w / total);
+  }
+}
+
+// The lowest of the threads' maxima that at least k of them reach (to 8 bins).
+__device__ __forceinline__ float top_k_low(Lds& s, const Weight& weight, float mine, int k) {
+  constexpr int N = kBins / 8;
+  const int tid = threadIdx.x;
+  if (tid < N) s.count[tid] = 0;
+  __syncthreads();
+  const int b = weight.bin(mine);
+  if (b < kBins) atomicAdd(&s.count[b / 8], 1u);
+  __syncthreads();
+  if (tid < 64) {
+    const uint4 c = *reinterpret_cast<const uint4*>(&s.count[4 * tid]);
+    uint32_t x = c.x + c.y + c.z + c.w;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t y = __shfl_up(x, d, 64);
+      if (tid >= d) x += y;
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(x >= (uint32_t)k);
+    if (tid == 0) {
+      s.found = kBins;
+      s.lo = 0xFFFFFFFFu;
+    }
+    if (m && tid == __builtin_ctzll(m)) {
+      uint32_t run = x - c.w - c.z - c.y;  // with the first of the four
+      int at = 0;
+      if (run < (uint32_t)k) { run += c.y; at = 1; }
+      if (at == 1 && run < (uint32_t)k) { run += c.z; at = 2; }
+      if (at == 2 && run < (uint32_t)k) at = 3;
+      s.found = 8 * (4 * tid + at) + 7;
+    }
+  }
+  __syncthreads();
+  const int cut = s.found;
+  if (cut == kBins) return -FLT_MAX;  // fewer hold a token of weight: every one
+  if (b <= cut) atomicMin(&s.lo, key_of(mine));
+  __syncthreads();
+  return value_of_key(s.lo);
 }
 
 // A row's own workgroup: the whole row, or with SLICED what its slices leave.
@@ -1088,15 +1198,16 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
   const int w0 = min(wave * per, row.vectors), w1 = min((wave + 1) * per, row.vectors);
   const RowParams q(a, r);
 
+  fill_powers<kThreads>(s.power);
   // ---- the max, and its first index
   float mine = -INFINITY;
-  Weight weight;
+  float top;
   int first;
-  if constexpr (SLICED) {
-    row_top(sa, r, weight.top, first);
+  if (SLICED && q.way != Way::kTopK) {
+    row_top(sa, r, top, first);
   } else {
     int at = -1;
-    row.walk(w0, w1, [&](float v, int i) {
+    row.template walk<true>(w0, w1, [&](float v, int i) {
       if (v > mine) {
         mine = v;
         at = i;
@@ -1109,12 +1220,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
       s.wave_i[wave] = at;
     }
     __syncthreads();
-    weight.top = s.wave_f[0];
+    top = s.wave_f[0];
     first = s.wave_i[0];
 #pragma unroll
     for (int w = 1; w < kWaves; w++)
-      if (s.wave_f[w] > weight.top) {
-        weight.top = s.wave_f[w];
+      if (s.wave_f[w] > top) {
+        top = s.wave_f[w];
         first = s.wave_i[w];
       }
   }
@@ -1125,9 +1236,9 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
     }
     return;
   }
-  weight.per = 1.4426950408889634 / (double)q.T;
-  weight.bins = 2.f * kBinsPerLog2 * (float)weight.per;
-  weight.limit = kBins;
+  __syncthreads();
+  Weight weight(top, q.T, s.power);
+  weight.set_bins(kBinsPerLog2, kBins);
   const double fixed = fixed_point(a.V);
 
   int token = -1;
@@ -1135,11 +1246,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
   int n = kList + 1;      // listed tokens
   double all = 0.0;       // the total that top-p is a share of (top-k: the list's)
   double below = 0.0;     // weight (where top-k acts, number) of the tokens before the listed
+  bool ready = false;     // the whole row's histogram is there
   bool slices = false;    // the row's weight is in its slices, the list only its last part
-  if constexpr (SLICED) {
-    if (q.way == Way::kTopK) {
-      n = join_lists(sa, r, s);
-    } else if (q.way == Way::kNucleus || q.way == Way::kRank) {
+  if (q.way == Way::kTopK) {
+    const float low = top_k_low(s, weight, mine, q.k);
+    n = collect<true>(row, s, [&](float v, int) { return v >= low; });
+  } else if constexpr (SLICED) {
+    if (q.way == Way::kNucleus || q.way == Way::kRank) {
       const SliceInfo info = sa.info[r];
       n = join_lists(sa, r, s);
       all = info.all;
@@ -1149,36 +1262,36 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
       n = 0;
       slices = true;
     }
-  } else if (q.way == Way::kTopK) {
-    // the k-th largest of the threads' maxima, to a bin
-    clear_histogram(s);
-    const int b = weight.bin(mine);
-    if (b < kBins) atomicAdd(&s.count[b], 1u);
-    __syncthreads();
-    const int cut = find_bin<true>(s, (uint32_t)q.k, 0.0, 0.0).bin;
-    // (kBins: fewer than k threads hold a token of weight)
-    n = gather(row, s, [&](float v, int) { return weight.bin(v) <= min(cut, kBins - 1); });
   } else if (q.way == Way::kNucleus) {
     const double least = q.least(a.V);
     clear_histogram(s);
     double x = 0.0;
     row.walk(w0, w1, [&](float v, int) {
-      const double w = weight.of(v);
+      int e;
+      const double w = weight.of(v, e);
       x += w;
-      const int b = weight.bin(v);
+      const int b = weight.bin_of(e);
       if (w >= least && b < kBins) {
         atomicAdd(&s.count[b], 1u);
-        atomicAdd(&s.mass[b], (unsigned long long)(w * fixed + 0.5));
+        atomicAdd(&s.mass[b], to_fixed(w, fixed));
       }
     });
     block_scan(x, s.wave_d, all);
+    ready = true;
     // (a little beyond p: the fixed-point sums are rounded)
     const BinAt b = find_bin<false>(s, 0, (double)q.p * all * (1.0 + 1e-9), 1.0 / fixed);
-    if (b.bin < kBins && b.before + b.in <= (uint32_t)kList)
-      n = gather(row, s, [&](float v, int) { return weight.bin(v) <= b.bin; });
+    if (b.bin < kBins && b.before + b.in <= (uint32_t)kList) {
+      const float low = value_of_key(lowest_key(weight, b.bin));
+      n = collect<true>(row, s, [&](float v, int) { return v >= low; });
+    }
+  }
+  if (n <= 64 && !slices) {
+    if (wave == 0) finish_few(a, r, q, weight, n, all, s);
+    return;
   }
   if (n <= kList) {
     const int i = threadIdx.x;
+    sort_list(s, n);
     if (i == 0) {
       s.found = kList;
       s.lo = 0;
@@ -1194,7 +1307,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
     }
     if (q.has_k && q.has_p) block_scan(in ? w : 0.0, s.wave_d, all);
     if (in && q.has_p) in = below + above < (double)q.p * all || (rank == 0 && below == 0.0);
-    if (in) in = w >= q.min_p;
+    if (in) in = w >= q.min_p && w > 0.0;
     if (!slices) {
       const double upto = block_scan(in ? w : 0.0, s.wave_d, total);
       const double target = q.u * total;
@@ -1248,12 +1361,11 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
       }
       const int sp = (row.vectors + sa.S - 1) / sa.S;
       const int v0 = min(max(at, 0) * sp, row.vectors), v1 = min(v0 + sp, row.vectors);
-      const Weight bins = slice_weight(q, weight.top, a.V);
-      const int lo = totals ? 0 : sa.info[r].lo;
+      const float high = totals ? INFINITY : sa.info[r].high;
       const Found f = find_within(row, v0, v1, base, target, s, [&](float v, int idx) {
         const double y = weight.of(v);
         if (totals) return y >= q.min_p ? y : 0.0;
-        return bins.bin(v) < lo || kept.has(key_of(v), idx) ? y : 0.0;
+        return v > high || kept.has(key_of(v), idx) ? y : 0.0;
       });
       token = f.index;
       w_token = f.f;
@@ -1262,10 +1374,12 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
     Kept kept;
     if (q.has_k) kept = last_kept<true>(row, weight, kept, (uint32_t)q.k, 0.0, fixed, s);
     if (q.has_p) {
-      double x = 0.0;
-      row.walk(w0, w1, [&](float v, int i) { x += kept.has(key_of(v), i) ? weight.of(v) : 0.0; });
-      block_scan(x, s.wave_d, all);
-      kept = last_kept<false>(row, weight, kept, 0u, (double)q.p * all, fixed, s);
+      if (!ready) {
+        double x = 0.0;
+        row.walk(w0, w1, [&](float v, int i) { x += kept.has(key_of(v), i) ? weight.of(v) : 0.0; });
+        block_scan(x, s.wave_d, all);
+      }
+      kept = last_kept<false>(row, weight, kept, 0u, (double)q.p * all, fixed, s, ready);
     }
     const Found f = find_index<true>(row, q.u, s, [&](float v, int i) {
       if (!kept.has(key_of(v), i)) return 0.0;
@@ -1286,17 +1400,19 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
 
 struct Layout {
   int S = 1;  // 1: no slices
-  size_t thread_top = 0, first = 0, total = 0, mass = 0, listed = 0, list = 0, info = 0,
+  size_t first = 0, total = 0, mass = 0, listed = 0, list = 0, info = 0,
          arrived = 0, bytes = 0;
 };
 
-// Some 1024 slices over all rows, of 4096 tokens or more.
+// Some 1024 slices over all rows, 16 of a row at most, from 32768 tokens on:
+// below, four launches cost what they save (one row of 32000, no filter 22 us
+// whole / 25 in slices, k = 50 17 / 25; of 128256 55 / 28, 24 / 28, p = 0.9 222 /
+// 50; 192 rows of 128256 68 / 75, 42 / 48, 246 / 120).
 Layout layout_of(int rows, int V) {
   Layout l;
   int64_t S = (1024 + (int64_t)rows - 1) / rows;
-  S = S < V / 4096 ? S : V / 4096;
   S = S < kMaxSlices ? S : kMaxSlices;
-  if (S < 2) return l;
+  if (V < 32768 || S < 2) return l;
   l.S = (int)S;
   const size_t n = (size_t)rows * S;
   size_t at = 0;
@@ -1307,7 +1423,6 @@ Layout layout_of(int rows, int V) {
   };
   put(n * 4);  // top
   l.first = put(n * 4);
-  l.thread_top = put(n * 4 * kSliceThreads);
   l.total = put(n * 8);
   l.mass = put(n * 8 * kSliceBins);
   l.listed = put(n * 4);
@@ -1373,7 +1488,6 @@ int sde_sample(const void* d_logits, int64_t row_stride, int dtype, int n_rows, 
     char* w = static_cast<char*>(d_workspace);
     sa.top = reinterpret_cast<float*>(w);
     sa.first = reinterpret_cast<int*>(w + l.first);
-    sa.thread_top = reinterpret_cast<float*>(w + l.thread_top);
     sa.total = reinterpret_cast<double*>(w + l.total);
     sa.mass = reinterpret_cast<unsigned long long*>(w + l.mass);
     sa.listed = reinterpret_cast<uint32_t*>(w + l.listed);

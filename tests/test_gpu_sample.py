@@ -240,8 +240,8 @@ def test_refusals(gpu):
         args.update(bad)
         with pytest.raises(error):
             sample(**args)
-    y = torch.zeros(2, 32000, device="cuda")
-    need = sample_workspace_size(2, 32000)
+    y = torch.zeros(2, 40000, device="cuda")
+    need = sample_workspace_size(2, 40000)
     assert need > 0 and sample_workspace_size(2, 50) == 0
     ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
     sample(y, u[:2], workspace=ws)

@@ -32,28 +32,23 @@ _DTYPES = {torch.float32: _native.SDE_F32, torch.float16: _native.SDE_F16,
            torch.bfloat16: _native.SDE_BF16}
 
 
-class _On:
-    """The buffers' device made current for a call where it is not already
-    (streams and launches belong to the current device)."""
-
-    def __init__(self, device):
-        self.guard = None
-        if device.index != (_raw_device() if _raw_device else torch.cuda.current_device()):
-            self.guard = torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_current = _raw_device if _raw_device is not None else torch.cuda.current_device
 
 
-def _rows(t, name: str, n: int, width: int, dtype, device) -> int:
+def _plain(t, dtype, shape: tuple, dev: int) -> bool:
+    """Whether t is a plain contiguous tensor of this type and shape on GPU `dev`
+    (a call's usual operand, told in one pass)."""
+    return (type(t) is torch.Tensor and t.dtype is dtype and t.shape == shape
+            and t.get_device() == dev and t.is_contiguous())
+
+
+def _rows(t, name: str, n: int, width: int, dtype, dev: int) -> int:
     """Checks rows [n][width] of `dtype` with neighbouring elements; their stride."""
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype:
-        raise TypeError(f"{name} must be a {dtype} tensor on {device}")
+    if _plain(t, dtype, (n, width), dev):
+        return width
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != dev \
+            or t.dtype != dtype:
+        raise TypeError(f"{name} must be a {dtype} tensor on cuda:{dev}")
     if t.shape != (n, width):
         raise ValueError(f"{name} must have shape {(n, width)}, got {tuple(t.shape)}")
     s = t.stride()
@@ -62,30 +57,46 @@ def _rows(t, name: str, n: int, width: int, dtype, device) -> int:
     return s[0] if n > 1 else max(s[0], width)
 
 
-def _ints(t, name: str, n: int, device) -> None:
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.int32:
-        raise TypeError(f"{name} must be an int32 tensor on {device}")
-    if t.shape != (n,) or not t.is_contiguous():
+def _values(t, name: str, n: int, dtype, dev: int) -> int:
+    """Checks n neighbouring values of `dtype`; their address."""
+    if not _plain(t, dtype, (n,), dev):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != dev \
+                or t.dtype != dtype:
+            raise TypeError(f"{name} must be a {dtype} tensor on cuda:{dev}")
         raise ValueError(f"{name} must be contiguous with shape {(n,)}, got {tuple(t.shape)}")
+    return t.data_ptr()
 
 
 def _pool(pool, tables, kv_dim: int) -> BatchPool:
-    if not isinstance(pool, torch.Tensor) or pool.device.type != "cuda" \
+    if not isinstance(pool, torch.Tensor) or not pool.is_cuda \
             or pool.dtype not in (torch.float16, torch.int16):
         raise TypeError("pool must be a CUDA float16 (or int16 bits) tensor")
-    if pool.dim() != 4 or pool.shape[1] != 2 or pool.shape[3] != kv_dim \
-            or not pool.is_contiguous():
+    ps = pool.shape
+    if len(ps) != 4 or ps[1] != 2 or ps[3] != kv_dim or not pool.is_contiguous():
         raise ValueError(f"pool must be contiguous [blocks][2][block_size][{kv_dim}], got "
-                         f"{tuple(pool.shape)}")
-    if not isinstance(tables, torch.Tensor) or tables.device != pool.device \
-            or tables.dtype != torch.int32:
+                         f"{tuple(ps)}")
+    if not isinstance(tables, torch.Tensor) or not tables.is_cuda \
+            or tables.get_device() != pool.get_device() or tables.dtype != torch.int32:
         raise TypeError(f"tables must be an int32 tensor on {pool.device}")
-    if tables.dim() != 2 or (tables.shape[1] > 1 and tables.stride(1) != 1) \
-            or (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]):
-        raise ValueError("tables must be [requests][blocks] with neighbouring entries")
+    if tables.dim() != 2:
+        raise ValueError("tables must be [requests][blocks]")
     n, blocks = tables.shape
-    return BatchPool(pool.data_ptr(), tables.data_ptr(), pool.shape[0], pool.shape[2], kv_dim, n,
-                     blocks, tables.stride(0) if n > 1 else blocks)
+    stride = blocks
+    if not tables.is_contiguous():
+        s = tables.stride()
+        if (blocks > 1 and s[1] != 1) or (n > 1 and s[0] < blocks):
+            raise ValueError("tables must be [requests][blocks] with neighbouring entries")
+        stride = s[0] if n > 1 else blocks
+    return BatchPool(pool.data_ptr(), tables.data_ptr(), ps[0], ps[2], kv_dim, n, blocks, stride)
+
+
+def _new(shape: tuple, dtype, device, stream, zero: bool = False) -> torch.Tensor:
+    """A new tensor that belongs to the call's stream: filled there, and its
+    memory free for other uses only behind the call."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _new(shape, dtype, device, None, zero)
+    return (torch.zeros if zero else torch.empty)(shape, dtype=dtype, device=device)
 
 
 def _workspace(given: Optional[torch.Tensor], need: int, device, stream):
@@ -93,9 +104,7 @@ def _workspace(given: Optional[torch.Tensor], need: int, device, stream):
     if given is None:
         if need == 0:
             return None, 0, None
-        given = torch.empty(need, dtype=torch.uint8, device=device)
-        if stream is not None:
-            given.record_stream(stream)
+        given = _new((need,), torch.uint8, device, stream)
         return given.data_ptr(), need, given
     if given.device != device or not given.is_contiguous():
         raise ValueError(f"workspace must be a contiguous tensor on {device}")
@@ -115,32 +124,37 @@ def batch_append(pool: torch.Tensor, tables: torch.Tensor, seq: torch.Tensor, po
     With q, [T][nh*dph] of the same type, its rotation goes to q_out (allocated
     when None; q itself: in place) and is returned; k_out takes the rotated k as
     well.  Rows may be slices of a fused projection."""
-    d = _pool(pool, tables, nkv * dph)
-    dev, T = pool.device, seq.shape[0]
-    dtype = _DTYPES.get(k.dtype)
+    kvd, dt = nkv * dph, k.dtype
+    d = _pool(pool, tables, kvd)
+    dev, T = pool.get_device(), seq.shape[0]
+    dtype = _DTYPES.get(dt)
     if dtype is None:
-        raise TypeError(f"k must be float32, float16 or bfloat16, got {k.dtype}")
-    _ints(seq, "seq", T, dev)
-    _ints(pos, "pos", T, dev)
-    ks = _rows(k, "k", T, nkv * dph, k.dtype, dev)
-    vs = _rows(v, "v", T, nkv * dph, k.dtype, dev)
+        raise TypeError(f"k must be float32, float16 or bfloat16, got {dt}")
+    if dev != _current():
+        with torch.cuda.device(dev):
+            return batch_append(pool, tables, seq, pos, k, v, nh, nkv, dph, theta, scaling_type,
+                                scaling_factor, rotate, q, q_out, k_out, stream)
+    sp = _values(seq, "seq", T, torch.int32, dev)
+    pp = _values(pos, "pos", T, torch.int32, dev)
+    ks = _rows(k, "k", T, kvd, dt, dev)
+    vs = _rows(v, "v", T, kvd, dt, dev)
+    qp = qop = kop = None
     qs = qos = kos = 0
     if q is not None:
-        qs = _rows(q, "q", T, nh * dph, k.dtype, dev)
+        qs = _rows(q, "q", T, nh * dph, dt, dev)
         if q_out is None:
-            q_out = torch.zeros(T, nh * dph, dtype=q.dtype, device=dev)
-        qos = _rows(q_out, "q_out", T, nh * dph, k.dtype, dev)
+            q_out = _new((T, nh * dph), dt, pool.device, stream, zero=True)
+        qos = _rows(q_out, "q_out", T, nh * dph, dt, dev)
+        qp, qop = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out needs q")
     if k_out is not None:
-        kos = _rows(k_out, "k_out", T, nkv * dph, k.dtype, dev)
+        kos = _rows(k_out, "k_out", T, kvd, dt, dev)
+        kop = k_out.data_ptr()
     rope = ctypes.byref(RopeConfig(theta, scaling_type, scaling_factor)) if rotate else None
-    with _On(dev):
-        check(_native.load().sde_batch_append(
-            ctypes.byref(d), seq.data_ptr(), pos.data_ptr(), T, dtype, k.data_ptr(), ks,
-            v.data_ptr(), vs, None if k_out is None else k_out.data_ptr(), kos,
-            None if q is None else q.data_ptr(), qs, None if q is None else q_out.data_ptr(), qos,
-            nh, nkv, dph, rope, _stream(stream)), "batch_append")
+    check(_native.load().sde_batch_append(
+        ctypes.byref(d), sp, pp, T, dtype, k.data_ptr(), ks, v.data_ptr(), vs, kop, kos, qp, qs,
+        qop, qos, nh, nkv, dph, rope, _stream(stream)), "batch_append")
     return q_out
 
 
@@ -163,25 +177,29 @@ def batch_attention(q: torch.Tensor, pool: torch.Tensor, tables: torch.Tensor,
     (batch_attention_workspace_size bytes) is taken from torch's allocator when
     None."""
     d = _pool(pool, tables, nkv * dph)
-    dev, n = pool.device, tables.shape[0]
-    dtype = _DTYPES.get(q.dtype)
+    dev, n, dt, width = pool.get_device(), d.n_seqs, q.dtype, nh * dph
+    dtype = _DTYPES.get(dt)
     if dtype is None:
-        raise TypeError(f"q must be float32, float16 or bfloat16, got {q.dtype}")
-    _ints(lens, "lens", n, dev)
-    qs = _rows(q, "q", n * n_queries, nh * dph, q.dtype, dev)
+        raise TypeError(f"q must be float32, float16 or bfloat16, got {dt}")
+    if dev != _current():
+        with torch.cuda.device(dev):
+            return batch_attention(q, pool, tables, lens, nh, nkv, dph, n_queries, max_len, out,
+                                   workspace, stream)
+    lp = _values(lens, "lens", n, torch.int32, dev)
+    qs = _rows(q, "q", n * n_queries, width, dt, dev)
     if max_len is None:
         max_len = d.max_blocks * d.block_size
-    with _On(dev):
-        if out is None:
-            out = torch.empty(n * n_queries, nh * dph, dtype=q.dtype, device=dev)
-        os = _rows(out, "out", n * n_queries, nh * dph, q.dtype, dev)
-        lib = _native.load()
-        ptr, size, workspace = _workspace(
-            workspace, lib.sde_batch_attention_workspace_size(n, nh, nkv, dph, n_queries, max_len,
-                                                              d.block_size), dev, stream)
-        check(lib.sde_batch_attention(
-            ctypes.byref(d), lens.data_ptr(), n_queries, max_len, dtype, q.data_ptr(), qs,
-            out.data_ptr(), os, nh, nkv, dph, ptr, size, _stream(stream)), "batch_attention")
+    if out is None:
+        out, os = _new((n * n_queries, width), dt, pool.device, stream), width
+    else:
+        os = _rows(out, "out", n * n_queries, width, dt, dev)
+    lib = _native.load()
+    ptr, size, workspace = _workspace(
+        workspace, lib.sde_batch_attention_workspace_size(n, nh, nkv, dph, n_queries, max_len,
+                                                          d.block_size), pool.device, stream)
+    check(lib.sde_batch_attention(ctypes.byref(d), lp, n_queries, max_len, dtype, q.data_ptr(), qs,
+                                  out.data_ptr(), os, nh, nkv, dph, ptr, size, _stream(stream)),
+          "batch_attention")
     return out
 
 
@@ -199,21 +217,24 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: 
     dtype = _DTYPES.get(q.dtype)
     if dtype is None or dtype == _native.SDE_F32:
         raise TypeError(f"q must be float16 or bfloat16, got {q.dtype}")
-    dev, T = q.device, q.shape[0]
-    qs = _rows(q, "q", T, nh * dph, q.dtype, dev)
-    ks = _rows(k, "k", T, nkv * dph, q.dtype, dev)
-    vs = _rows(v, "v", T, nkv * dph, q.dtype, dev)
+    dt, dev, T = q.dtype, q.get_device(), q.shape[0]
+    if dev != _current():
+        with torch.cuda.device(dev):
+            return prompt_attention(q, k, v, starts, nh, nkv, dph, out, stream)
+    qs = _rows(q, "q", T, nh * dph, dt, dev)
+    ks = _rows(k, "k", T, nkv * dph, dt, dev)
+    vs = _rows(v, "v", T, nkv * dph, dt, dev)
     if not isinstance(starts, torch.Tensor) or starts.dim() != 1 or starts.shape[0] < 1:
         raise ValueError("starts must have one entry per sequence and one for the end")
-    _ints(starts, "starts", starts.shape[0], dev)
-    with _On(dev):
-        if out is None:
-            out = torch.zeros(T, nh * dph, dtype=q.dtype, device=dev)
-        os = _rows(out, "out", T, nh * dph, q.dtype, dev)
-        check(_native.load().sde_prompt_attention(
-            starts.data_ptr(), starts.shape[0] - 1, T, dtype, q.data_ptr(), qs, k.data_ptr(), ks,
-            v.data_ptr(), vs, out.data_ptr(), os, nh, nkv, dph, _stream(stream)),
-            "prompt_attention")
+    n = starts.shape[0]
+    sp = _values(starts, "starts", n, torch.int32, dev)
+    if out is None:
+        out, os = _new((T, nh * dph), dt, q.device, stream, zero=True), nh * dph
+    else:
+        os = _rows(out, "out", T, nh * dph, dt, dev)
+    check(_native.load().sde_prompt_attention(
+        sp, n - 1, T, dtype, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
+        os, nh, nkv, dph, _stream(stream)), "prompt_attention")
     return out
 
 
@@ -241,31 +262,27 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Optional[torch.Te
     dtype = _DTYPES.get(logits.dtype)
     if dtype is None:
         raise TypeError(f"logits must be float32, float16 or bfloat16, got {logits.dtype}")
-    dev, (n, V) = logits.device, logits.shape
+    dev, (n, V) = logits.get_device(), logits.shape
+    if dev != _current():
+        with torch.cuda.device(dev):
+            return sample(logits, u, temperature, top_k, top_p, min_p, tokens, probs, workspace,
+                          stream)
+    f32, i32 = torch.float32, torch.int32
     stride = _rows(logits, "logits", n, V, logits.dtype, dev)
-    for t, name, want in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
-                          (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
-                          (min_p, "min_p", torch.float32), (tokens, "tokens", torch.int32),
-                          (probs, "probs", torch.float32)):
-        if t is None and name != "u":
-            continue
-        if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != want:
-            raise TypeError(f"{name} must be a {want} tensor on {dev}")
-        if t.shape != (n,) or not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous with shape {(n,)}, got {tuple(t.shape)}")
-    with _On(dev):
-        if tokens is None:
-            tokens = torch.empty(n, dtype=torch.int32, device=dev)
-        if probs is None:
-            probs = torch.empty(n, dtype=torch.float32, device=dev)
-        lib = _native.load()
-        ptr, size, workspace = _workspace(workspace, lib.sde_sample_workspace_size(n, V), dev,
-                                          stream)
-        check(lib.sde_sample(
-            logits.data_ptr(), stride, dtype, n, V, u.data_ptr(),
-            None if temperature is None else temperature.data_ptr(),
-            None if top_k is None else top_k.data_ptr(),
-            None if top_p is None else top_p.data_ptr(),
-            None if min_p is None else min_p.data_ptr(), tokens.data_ptr(), probs.data_ptr(),
-            ptr, size, _stream(stream)), "sample")
+    up = _values(u, "u", n, f32, dev)
+    tp = None if temperature is None else _values(temperature, "temperature", n, f32, dev)
+    kp = None if top_k is None else _values(top_k, "top_k", n, i32, dev)
+    pp = None if top_p is None else _values(top_p, "top_p", n, f32, dev)
+    mp = None if min_p is None else _values(min_p, "min_p", n, f32, dev)
+    if tokens is None:
+        tokens = _new((n,), i32, logits.device, stream)
+    if probs is None:
+        probs = _new((n,), f32, logits.device, stream)
+    lib = _native.load()
+    ptr, size, workspace = _workspace(workspace, lib.sde_sample_workspace_size(n, V),
+                                      logits.device, stream)
+    check(lib.sde_sample(
+        logits.data_ptr(), stride, dtype, n, V, up, tp, kp, pp, mp,
+        _values(tokens, "tokens", n, i32, dev), _values(probs, "probs", n, f32, dev), ptr, size,
+        _stream(stream)), "sample")
     return tokens, probs

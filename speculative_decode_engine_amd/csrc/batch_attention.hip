@@ -8,10 +8,10 @@
 // What bounds it is the cache: each K and V byte is read once and serves the
 // G = nh / nkv query heads of its KV head (times m queries), a few operations
 // per byte.  So:
-//  * a workgroup takes (request, KV head, group of 16 rows, partition of the
-//    positions); a wave takes every kWaves-th tile of 32 positions of it on
-//    its own -- own buffers, no barrier in the loop -- and the waves' sums meet
-//    in LDS at the end;
+//  * a workgroup takes (request, KV head, up to 48 rows, partition of the
+//    positions); each of its waves takes every W-th tile of 32 positions of it
+//    on its own -- own buffers, no barrier in the loop -- and the waves' sums
+//    meet in LDS at the end;
 //  * K and V go from memory straight into LDS, two tiles ahead; a buffer is
 //    filled again as soon as its tile is in registers, so some 24 KiB per
 //    wave are in flight at head size 128 while it computes;
@@ -26,6 +26,13 @@
 //    are the weights, which keeps 22 bits of them; sums are fp32.  (fp16 and
 //    bf16 q are their hi parts.)
 //  * the max is raised only when a logit is 2^8 above it.
+//
+// Measured on MI355X (graph replays over three inputs), 32/8 heads of 128 where
+// not said: 96 requests up to 8K, bf16, 1.64 GB: 323 us, 5.1 TB/s (a copy of 4 GiB
+// runs at 4.7); 16 up to 4K, 149 MB: 39 us, 3.8 TB/s; one of 32K: 35 us, 3.9; the
+// 5-query verify of 3 up to 32K, 28/4 heads, 144 MB: 55 us, the combine's 8 in it.
+// Short of the bandwidth there: some 4 us pass before a workgroup's first tile is
+// there (length and table, then K), and partitions end unevenly.
 #include <algorithm>
 #include <cmath>
 
@@ -40,7 +47,7 @@ using attn::h8_t;
 using attn::lds_s4_t;
 using attn::s4_t;
 
-constexpr int kRows = 16;       // rows (query, head in group) of a workgroup
+constexpr int kRows = 16;       // rows (query, head in group) of a group: one MFMA's
 constexpr int kTok = 32;        // positions per tile
 constexpr int kTable = 1024;    // block table entries of a partition in LDS
 constexpr int kMaxQueries = 64;
@@ -71,7 +78,6 @@ struct Shape {
   static constexpr int TILEB = kTok * ROWB;
   static constexpr int NL = TILEB / 1024;  // loads per wave and tile of K (or V)
   static constexpr int RING = 4 * TILEB;   // two tiles of K and V
-  static constexpr int WAVES = DP > 128 ? 2 : 4;
 };
 
 // Which unit of token t's row lies at place u: u ^ swizzle(t).  16 tokens read
@@ -179,14 +185,14 @@ __device__ __forceinline__ int64_t row_at(const BatchArgs& a, int b, int kvh, in
 }
 
 // FULL: the head has DP features (else fewer: the rest of each staged row is
-// zero).
-template <int DP, bool FULL>
-__global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(BatchArgs a) {
+// zero).  W waves, RG row groups, whose rows share every tile's operands.
+template <int DP, bool FULL, int W, int RG>
+__global__ __launch_bounds__(64 * W) void batch_attention_kernel(BatchArgs a) {
   using Sh = Shape<DP>;
-  constexpr int W = Sh::WAVES;
   __shared__ __attribute__((aligned(1024))) char ring[W * Sh::RING];
   __shared__ int32_t tab[kTable];
-  __shared__ float2 sums[W][kRows];
+  __shared__ float2 sums[W][RG * kRows];
+  __shared__ int first_bad[DP], any_bad;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63;
@@ -198,31 +204,17 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
   const int kvh = n - u * a.nkv;
   n = u;
   u = wave_uniform(n / a.row_groups);
-  const int r0 = (n - u * a.row_groups) * kRows;
+  const int r0 = (n - u * a.row_groups) * (RG * kRows);
   const int b = wave_uniform(u / a.n_parts);
   const int part = u - b * a.n_parts;
-  const int rows = min(kRows, a.R - r0);
+  const int rows = min(RG * kRows, a.R - r0);
+  const int groups = (rows + kRows - 1) / kRows;
 
   // Length, table entries and q are all on their way before any is used.
   const int p0 = part * a.part_tokens;
   const int b0 = wave_uniform(p0 / a.bs);
   const int n_tab = min(wave_uniform((p0 + a.part_tokens - 1) / a.bs) + 1, a.max_blocks) - b0;
   const int len = min(max(a.lens[b], 0), a.max_len);
-  const int32_t* const trow = a.tables + (int64_t)b * a.table_stride + b0;
-  for (int i = tid; i < n_tab; i += 64 * W) tab[i] = trow[i];
-  const bool real = l16 < rows;
-  const int row = r0 + l16;
-  float qx[Sh::KS][8];
-  {
-    // (rows beyond the group's read its first: their logits are masked)
-    const int64_t at = row_at(a, b, kvh, real ? row : r0, a.q_stride);
-    if (a.dtype == SDE_F32)
-      load_q<f32_elem>(a.q, at, grp, a.dph, a.wide_q, qx);
-    else if (a.dtype == SDE_F16)
-      load_q<f16_elem>(a.q, at, grp, a.dph, a.wide_q, qx);
-    else
-      load_q<bf16_elem>(a.q, at, grp, a.dph, a.wide_q, qx);
-  }
   const int p1 = min(p0 + a.part_tokens, len);
   if (p0 >= p1) {  // nothing here (the combine leaves this partition out)
     if (a.n_parts == 1)
@@ -233,25 +225,47 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
       }
     return;
   }
+  const int32_t* const trow = a.tables + (int64_t)b * a.table_stride + b0;
+  for (int i = tid; i < n_tab; i += 64 * W) tab[i] = trow[i];
+  for (int i = tid; i < DP; i += 64 * W) first_bad[i] = INT32_MAX;
+  if (tid == 0) any_bad = 0;
+
   // q scaled by a power of two to a largest element in [1, 2): any finite q
   // fits fp16's range, and the hi + lo split keeps 22 bits of it.
-  float mx = 0.f;
+  h8_t qh[RG][Sh::KS], ql[RG][Sh::KS];
+  float row_scale[RG];
+  int last[RG];  // the last position that this lane's row sees
 #pragma unroll
-  for (int ks = 0; ks < Sh::KS; ks++)
+  for (int g = 0; g < RG; g++) {
+    const int row = r0 + kRows * g + l16;
+    const bool real = kRows * g + l16 < rows;
+    last[g] = real ? len - a.m + row / a.G : -1;
+    // (rows beyond the group's read its first: their logits are masked)
+    float qx[Sh::KS][8];
+    const int64_t at = row_at(a, b, kvh, real ? row : r0, a.q_stride);
+    if (a.dtype == SDE_F32)
+      load_q<f32_elem>(a.q, at, grp, a.dph, a.wide_q, qx);
+    else if (a.dtype == SDE_F16)
+      load_q<f16_elem>(a.q, at, grp, a.dph, a.wide_q, qx);
+    else
+      load_q<bf16_elem>(a.q, at, grp, a.dph, a.wide_q, qx);
+    float mx = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qx[ks][e]));
-  mx = attn::groups_max(mx);
-  // (a row of zeros or with an infinity keeps its scale)
-  const int ex = mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0;
-  const float row_scale = ldexpf(a.scale, ex);
-  h8_t qh[Sh::KS], ql[Sh::KS];
+    for (int ks = 0; ks < Sh::KS; ks++)
 #pragma unroll
-  for (int ks = 0; ks < Sh::KS; ks++) {
+      for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qx[ks][e]));
+    mx = attn::groups_max(mx);
+    // (a row of zeros or with an infinity keeps its scale)
+    const int ex = mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0;
+    row_scale[g] = ldexpf(a.scale, ex);
 #pragma unroll
-    for (int e = 0; e < 8; e++) qx[ks][e] = ldexpf(qx[ks][e], -ex);
-    attn::split_h8(qx[ks], qh[ks], ql[ks]);
+    for (int ks = 0; ks < Sh::KS; ks++) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) qx[ks][e] = ldexpf(qx[ks][e], -ex);
+      attn::split_h8(qx[ks], qh[g][ks], ql[g][ks]);
+    }
   }
-  const bool lo_q = a.dtype == SDE_F32;   // fp16 and bf16 elements are their hi parts
+  const bool lo_q = a.dtype == SDE_F32;  // fp16 and bf16 elements are their hi parts
 
   int bad = 0;  // pages outside the pool: their positions are left out
   for (int i = tid; i <= wave_uniform((p1 - 1) / a.bs) - b0; i += 64 * W)
@@ -316,20 +330,26 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
     load_rows(prow, a.bs, lds0 + 3 * Sh::TILEB);
   }
 
-  const int qi = row / a.G;                       // the row's query
-  const int last = real ? len - a.m + qi : -1;    // and the last position it sees
-  const int all_see = len - a.m;                  // the last that every query sees
-  f4_t o[Sh::FB];
+  const int all_see = len - a.m;  // the last position that every query sees
+  f4_t o[RG][Sh::FB];
 #pragma unroll
-  for (int fb = 0; fb < Sh::FB; fb++) o[fb] = f4_t{0.f, 0.f, 0.f, 0.f};
+  for (int g = 0; g < RG; g++)
+#pragma unroll
+    for (int fb = 0; fb < Sh::FB; fb++) o[g][fb] = f4_t{0.f, 0.f, 0.f, 0.f};
   // Weights are 2^(logit - ref), ref = max - kWeightShift: below 2^15, and
   // fp16's quantum of their lo parts is 2^-32 of the largest.
-  float ref = 0.f, raise = -INFINITY, l = 0.f;
+  float ref[RG], raise[RG], l[RG];
+#pragma unroll
+  for (int g = 0; g < RG; g++) {
+    ref[g] = l[g] = 0.f;
+    raise[g] = -INFINITY;
+  }
   const int vt = 4 * grp + (l16 >> 2);  // transposed V reads: this lane's token
   const int vu = (l16 & 3) >> 1, vsub = 8 * (l16 & 1);
 
   for (int i = 0; i < nt; i++) {
-    const char* kst = mine + (i & 1) * 2 * Sh::TILEB;
+    char* const kst = mine + (i & 1) * 2 * Sh::TILEB;
+    char* const vst = kst + Sh::TILEB;
     const uint32_t dst = lds0 + (uint32_t)(i & 1) * 2 * Sh::TILEB;
     const int at0 = kTok * (wave + W * i);
     if (i + 1 < nt)
@@ -339,7 +359,7 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
     // (a long head's operands are read in halves, within the registers)
     constexpr bool kHalves = Sh::KS > 4;
     h8_t k8[kHalves ? 1 : 2][Sh::KS];
-    f4_t s[2], s2[2];
+    f4_t s[RG][2];
     auto read_k = [&](int h, h8_t(&k)[Sh::KS]) {
       const int t = 16 * h + l16;
 #pragma unroll
@@ -348,14 +368,19 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
             kst + t * Sh::ROWB + 16 * ((4 * ks + grp) ^ swizzle<DP>(t)));
     };
     auto logits = [&](int h, const h8_t(&k)[Sh::KS]) {
-      s[h] = s2[h] = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ks = 0; ks < Sh::KS; ks++)
-        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[ks], qh[ks], s[h], 0, 0, 0);
-      if (lo_q) {
+      for (int g = 0; g < RG; g++) {
+        if (g > 0 && g >= groups) break;
+        f4_t x = f4_t{0.f, 0.f, 0.f, 0.f}, y = f4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < Sh::KS; ks++)
-          s2[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[ks], ql[ks], s2[h], 0, 0, 0);
+          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[ks], qh[g][ks], x, 0, 0, 0);
+        if (lo_q) {
+#pragma unroll
+          for (int ks = 0; ks < Sh::KS; ks++)
+            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[ks], ql[g][ks], y, 0, 0, 0);
+        }
+        s[g][h] = x + y;
       }
     };
     read_k(0, k8[0]);
@@ -366,15 +391,12 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
     if (i + 2 < nt) load_rows(prow, 0, dst);
     if constexpr (!kHalves) logits(0, k8[0]);
     logits(1, k8[kHalves ? 0 : 1]);
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = (s[e >> 2][e & 3] + s2[e >> 2][e & 3]) * row_scale;
 
     // positions some row does not see, or past the end, or in no page
     const bool edge = bad || p0 + at0 + kTok - 1 > all_see;
-    uint32_t seen = 0xFF;  // bit e: position e of this lane exists
+    uint32_t there = 0xFF;  // bit e: position e of this lane exists
     if (edge) {
-      seen = 0;
+      there = 0;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const int at = at0 + 16 * (e >> 2) + 4 * grp + (e & 3);
@@ -383,33 +405,46 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
           int slot;
           in = in && page_of(base_rel + min(at, p1 - p0 - 1), slot) >= 0;
         }
-        seen |= in ? 1u << e : 0u;
-        x[e] = in && p0 + at <= last ? x[e] : -INFINITY;
+        there |= in ? 1u << e : 0u;
       }
     }
-    float top = x[0];
+    h8_t ph[RG], pl[RG];
 #pragma unroll
-    for (int e = 1; e < 8; e++) top = fmaxf(top, x[e]);
-    if (__builtin_amdgcn_ballot_w64(top > raise) != 0) {
-      top = attn::groups_max(top);
-      if (top > raise) {
-        // (a row's first logits: its sums are zero, and the factor too)
-        const float to = fmaxf(top - kWeightShift, raise == -INFINITY ? -INFINITY : ref);
-        const float f = raise == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to);
-        ref = to;
-        raise = to + kWeightShift + kLazyMax;
-        l *= f;
+    for (int g = 0; g < RG; g++) {
+      if (g > 0 && g >= groups) break;
+      float x[8];
 #pragma unroll
-        for (int fb = 0; fb < Sh::FB; fb++) o[fb] *= f;
+      for (int e = 0; e < 8; e++) x[e] = s[g][e >> 2][e & 3] * row_scale[g];
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          x[e] = (there >> e & 1) && p0 + at0 + 16 * (e >> 2) + 4 * grp + (e & 3) <= last[g]
+                     ? x[e]
+                     : -INFINITY;
       }
-    }
+      float top = x[0];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      x[e] = __builtin_amdgcn_exp2f(x[e] - ref);
-      l += x[e];
+      for (int e = 1; e < 8; e++) top = fmaxf(top, x[e]);
+      if (__builtin_amdgcn_ballot_w64(top > raise[g]) != 0) {
+        top = attn::groups_max(top);
+        if (top > raise[g]) {
+          // (a row's first logits: its sums are zero, and the factor too)
+          const float to = top - kWeightShift;
+          const float f = raise[g] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref[g] - to);
+          ref[g] = to;
+          raise[g] = to + kWeightShift + kLazyMax;
+          l[g] *= f;
+#pragma unroll
+          for (int fb = 0; fb < Sh::FB; fb++) o[g][fb] *= f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        x[e] = __builtin_amdgcn_exp2f(x[e] - ref[g]);
+        l[g] += x[e];
+      }
+      attn::split_h8(x, ph[g], pl[g]);
     }
-    h8_t ph, pl;
-    attn::split_h8(x, ph, pl);
 
     // outstanding after this tile's V: tile i + 1, and K of i + 2
     if (i + 2 < nt)
@@ -418,7 +453,40 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
       wait_loads<2 * Sh::NL>();
     else
       wait_loads<0>();
-    const char* vst = kst + Sh::TILEB;
+    if (edge) {
+      // What lies at positions that do not exist must not meet a weight of 0
+      // (0 x Inf): it becomes 0.  So does an element that is not finite at a
+      // position hidden from some row, and the rows that do see it are marked:
+      // by feature, the first such position.
+#pragma unroll 1
+      for (int j = 0; j < Sh::NL; j++) {
+        const int place = 64 * j + lane;
+        const int t = place / Sh::UNITS;
+        const int at = at0 + t;
+        bool in = at < p1 - p0;
+        if (bad && in) {
+          int slot;
+          in = page_of(base_rel + at, slot) >= 0;
+        }
+        uint4* const v = reinterpret_cast<uint4*>(vst + 16 * place);
+        const uint4 x = *v;
+        if (!in) {
+          *v = make_uint4(0, 0, 0, 0);
+        } else if (p0 + at > all_see && (attn::nonfinite_h2(x.x) | attn::nonfinite_h2(x.y) |
+                                         attn::nonfinite_h2(x.z) | attn::nonfinite_h2(x.w)) != 0) {
+          const int unit = (place - t * Sh::UNITS) ^ swizzle<DP>(t);
+          uint16_t* const e = reinterpret_cast<uint16_t*>(v);
+#pragma unroll 1
+          for (int k = 0; k < 8; k++)
+            if (attn::nonfinite_h2(e[k]) != 0) {
+              e[k] = 0;
+              atomicMin(&first_bad[8 * unit + k], p0 + at);
+              any_bad = 1;
+            }
+        }
+      }
+      wait_lds();
+    }
     typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
     u4_t v8[Sh::FB];
 #pragma unroll
@@ -434,74 +502,34 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
       }
     wait_lds();
     if (i + 2 < nt) load_rows(prow, a.bs, dst + Sh::TILEB);
-
-    if (edge) {
-      // What lies at positions that do not exist must not meet a weight of 0
-      // (0 x Inf): it becomes 0.  A non-finite element that some rows see and
-      // others do not takes a product per query.
-      uint32_t some = 0;  // bit e: hidden from a row of the workgroup
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (p0 + at0 + 16 * (e >> 2) + 4 * grp + (e & 3) > all_see) some |= 1u << e;
-      uint32_t hit = 0;
+    for (int g = 0; g < RG; g++) {
+      if (g > 0 && g >= groups) break;
 #pragma unroll
-      for (int d = 0; d < 4; d++) {
-        const uint32_t two = seen >> (2 * d);
-        const uint32_t keep = (two & 1 ? 0xFFFFu : 0u) | (two & 2 ? 0xFFFF0000u : 0u);
-        const uint32_t st = some >> (2 * d);
-        const uint32_t sm = (st & 1 ? 0xFFFFu : 0u) | (st & 2 ? 0xFFFF0000u : 0u);
+      for (int fb = 0; fb < Sh::FB; fb++)
+        o[g][fb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, v8[fb]), ph[g],
+                                                          o[g][fb], 0, 0, 0);
 #pragma unroll
-        for (int fb = 0; fb < Sh::FB; fb++) {
-          v8[fb][d] &= keep;
-          hit |= attn::nonfinite_h2(v8[fb][d] & sm);
-        }
-      }
-      if (__builtin_amdgcn_ballot_w64(hit != 0) != 0) {
-        const int i0 = r0 / a.G, i1 = (r0 + rows - 1) / a.G;
-#pragma unroll 1
-        for (int w = i0; w <= i1; w++) {
-          uint32_t keep[4];
-#pragma unroll
-          for (int d = 0; d < 4; d++) {
-            const int at = p0 + at0 + 16 * (d >> 1) + 4 * grp + 2 * (d & 1);
-            const int lim = len - a.m + w;
-            keep[d] = (at <= lim ? 0xFFFFu : 0u) | (at + 1 <= lim ? 0xFFFF0000u : 0u);
-          }
-#pragma unroll
-          for (int fb = 0; fb < Sh::FB; fb++) {
-            u4_t v = v8[fb];
-#pragma unroll
-            for (int d = 0; d < 4; d++) v[d] &= keep[d];
-            f4_t y = f4_t{0.f, 0.f, 0.f, 0.f};
-            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, v), ph, y, 0, 0, 0);
-            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, v), pl, y, 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[fb][e] += qi == w ? y[e] : 0.f;
-          }
-        }
-        continue;
-      }
+      for (int fb = 0; fb < Sh::FB; fb++)
+        o[g][fb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, v8[fb]), pl[g],
+                                                          o[g][fb], 0, 0, 0);
     }
-#pragma unroll
-    for (int fb = 0; fb < Sh::FB; fb++)
-      o[fb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, v8[fb]), ph, o[fb], 0,
-                                                     0, 0);
-#pragma unroll
-    for (int fb = 0; fb < Sh::FB; fb++)
-      o[fb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, v8[fb]), pl, o[fb], 0,
-                                                     0, 0);
   }
 
   // ---- the waves' sums meet in LDS (every tile has been read)
-  l = attn::groups_sum(l);
   constexpr int C = DP / 4;  // 16-byte units per row
-  static_assert(kRows * DP * 4 <= Sh::RING, "a wave's sums fit its ring");
+  static_assert(RG * kRows * DP * 4 <= Sh::RING, "a wave's sums fit its ring");
   float4* const mo = reinterpret_cast<float4*>(mine);
 #pragma unroll
-  for (int fb = 0; fb < Sh::FB; fb++)
-    mo[l16 * C + ((4 * fb + grp) ^ (l16 & 7))] =
-        make_float4(o[fb][0], o[fb][1], o[fb][2], o[fb][3]);
-  if (grp == 0) sums[wave][l16] = make_float2(raise == -INFINITY ? -INFINITY : ref, l);
+  for (int g = 0; g < RG; g++) {
+    const float lt = attn::groups_sum(l[g]);
+#pragma unroll
+    for (int fb = 0; fb < Sh::FB; fb++)
+      mo[(kRows * g + l16) * C + ((4 * fb + grp) ^ (l16 & 7))] =
+          make_float4(o[g][fb][0], o[g][fb][1], o[g][fb][2], o[g][fb][3]);
+    if (grp == 0)
+      sums[wave][kRows * g + l16] = make_float2(raise[g] == -INFINITY ? -INFINITY : ref[g], lt);
+  }
   __syncthreads();
   for (int i = tid; i < rows * C; i += 64 * W) {
     const int r = i / C, c = i - r * C;
@@ -525,6 +553,14 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
       y.z += z.z * f;
       y.w += z.w * f;
     }
+    if (any_bad) {
+      const int see = len - a.m + (r0 + r) / a.G;
+      const int* fb = &first_bad[4 * c];
+      y.x = fb[0] <= see ? NAN : y.x;
+      y.y = fb[1] <= see ? NAN : y.y;
+      y.z = fb[2] <= see ? NAN : y.z;
+      y.w = fb[3] <= see ? NAN : y.w;
+    }
     if (a.n_parts == 1) {
       const float inv = lt == 0.f ? 0.f : 1.f / lt;
       y.x *= inv;
@@ -542,29 +578,32 @@ __global__ __launch_bounds__(64 * Shape<DP>::WAVES) void batch_attention_kernel(
   }
 }
 
-// Joins a row's partitions, in order: one thread per (row, 4 features).
-__global__ __launch_bounds__(256) void batch_combine_kernel(BatchArgs a) {
-  const int C = a.dph / 4;
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const size_t kr = i / C;
-  if (kr >= (size_t)a.n_seqs * a.nkv * a.R) return;
-  const int c = (int)(i - kr * C);
-  const int bk = (int)(kr / a.R), row = (int)(kr - (size_t)bk * a.R);
+// Joins a row's partitions: a workgroup per row, kJoin of its threads side by
+// side over a 16-byte unit's partitions, whose sums meet in LDS in order.
+constexpr int kJoin = 8;
+
+__global__ __launch_bounds__(64 * kJoin) void batch_combine_kernel(BatchArgs a) {
+  __shared__ float4 part_y[kJoin][64];
+  __shared__ float2 part_ml[kJoin];
+  const int kr = blockIdx.x;
+  const int c = threadIdx.x & 63, j = threadIdx.x >> 6;
+  const int bk = kr / a.R, row = kr - bk * a.R;
   const int b = bk / a.nkv, kvh = bk - b * a.nkv;
   const int len = min(max(a.lens[b], 0), a.max_len);
   const int P = (len + a.part_tokens - 1) / a.part_tokens;
-  const float* acc = a.partials + kr * a.n_parts * a.dph + 4 * c;
+  const bool in = 4 * c < a.dph;
+  const float* acc = a.partials + (size_t)kr * a.n_parts * a.dph + (in ? 4 * c : 0);
   const float2* ml = reinterpret_cast<const float2*>(
                          a.partials + (size_t)a.n_seqs * a.nkv * a.R * a.n_parts * a.dph) +
-                     kr * a.n_parts;
+                     (size_t)kr * a.n_parts;
   float top = -INFINITY, l = 0.f;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < P; p0 += 4) {
+  for (int p0 = j; p0 < P; p0 += 4 * kJoin) {
     float2 v[4];
     float4 x[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const int p = min(p0 + k, P - 1);
+      const int p = min(p0 + k * kJoin, P - 1);
       v[k] = ml[p];
       x[k] = *reinterpret_cast<const float4*>(acc + (size_t)p * a.dph);
     }
@@ -580,7 +619,7 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchArgs a) {
     y.w *= old;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      if (p0 + k >= P) continue;
+      if (p0 + k * kJoin >= P) continue;
       const float f =
           v[k].x == -INFINITY ? (v[k].y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(v[k].x - top);
       l += v[k].y * f;
@@ -590,27 +629,64 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchArgs a) {
       y.w += x[k].w * f;
     }
   }
+  part_y[j][c] = y;
+  if (c == 0) part_ml[j] = make_float2(top, l);
+  __syncthreads();
+  if (j > 0 || !in) return;
+  top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kJoin; k++) top = fmaxf(top, part_ml[k].x);
+  l = 0.f;
+  y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < kJoin; k++) {
+    const float2 v = part_ml[k];
+    const float4 x = part_y[k][c];
+    const float f = v.x == -INFINITY ? (v.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(v.x - top);
+    l += v.y * f;
+    y.x += x.x * f;
+    y.y += x.y * f;
+    y.z += x.z * f;
+    y.w += x.w * f;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   store4(a.out, row_at(a, b, kvh, row, a.out_stride) + 4 * c,
          make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv), a.dtype, a.wide_out);
 }
 
 struct BatchPlan {
+  int per_group = 1;  // row groups of a workgroup
   int row_groups = 1, n_parts = 1, part_tokens = kTok;
 };
 
-// Positions per partition: enough partitions for some kFill workgroups over
-// all requests (each of which may be much shorter than max_len), none shorter
-// than kMinPart positions, and none longer than its table entries in LDS.
-constexpr int kFill = 2048;
-constexpr int kMinPart = 256;
+// Row groups of a workgroup: rows up to 48 together, so that K and V are read
+// once; as many as the registers hold without scratch, whose loads would wait
+// for the tiles' (two above head size 128, one above 192).
+int groups_per(int R, int dph) {
+  const int g = (R + kRows - 1) / kRows;
+  const int most = dph > 192 ? 1 : dph > 128 ? 2 : 3;
+  const int n = (g + most - 1) / most;
+  return (g + n - 1) / n;
+}
 
-BatchPlan batch_plan(int n_seqs, int nkv, int R, int max_len, int bs) {
+// Partitions.  With few (request, KV head, row group) units, some 640 workgroups
+// over max_len: at the requests' own lengths that is about the two per CU that
+// run at once.  Positions: 256 or more.  From a unit per CU on a partition only
+// evens out the requests' lengths: up to 4096 workgroups, over 512 positions or
+// more, from two units per CU on over 1024.  Measured on MI355X, us per call by
+// the number of workgroups aimed at (512 / 768 / 4096), 32/8 heads of 128: 16
+// requests up to 4K 41.1 / 39.1 / 45, one of 32K 35.6 / 36 / 45, the 5-query verify
+// of 3 up to 32K 55 / 66 / 90, 40 up to 2K 61.9 / 61 / 56.5, 96 up to 8K 367 / 367 /
+// 323; 128 up to 1K with 1024 positions at least 67, with 256 98.  No partition
+// has more table entries than fit LDS.
+BatchPlan batch_plan(int n_seqs, int nkv, int R, int dph, int max_len, int bs) {
   BatchPlan p;
-  p.row_groups = (R + kRows - 1) / kRows;
+  p.per_group = groups_per(R, dph);
+  p.row_groups = (R + kRows * p.per_group - 1) / (kRows * p.per_group);
   const int64_t units = std::max<int64_t>(1, (int64_t)n_seqs * nkv * p.row_groups);
-  int64_t tokens = ((int64_t)max_len + kFill / units) / std::max<int64_t>(1, kFill / units);
-  tokens = std::max<int64_t>(tokens, kMinPart);
+  const int64_t parts = std::max<int64_t>(1, (units < 256 ? 640 : 4096) / units);
+  int64_t tokens = ((int64_t)max_len + parts - 1) / parts;
+  tokens = std::max<int64_t>(tokens, units < 256 ? 256 : units < 512 ? 512 : 1024);
   tokens = std::min<int64_t>(tokens, (int64_t)(kTable - 2) * bs);
   tokens = std::min<int64_t>(tokens, 1 << 20);  // (page_of's division)
   tokens = std::max<int64_t>(tokens / kTok * kTok, kTok);
@@ -624,13 +700,29 @@ size_t batch_partial_bytes(const BatchPlan& p, int n_seqs, int nkv, int R, int d
                        : 0;
 }
 
-template <int DP>
-void launch(const BatchArgs& a, unsigned grid, hipStream_t s) {
-  const dim3 block(64 * Shape<DP>::WAVES);
+template <int DP, int W, int RG>
+void launch_groups(const BatchArgs& a, unsigned grid, hipStream_t s) {
   if (a.dph == DP)
-    batch_attention_kernel<DP, true><<<dim3(grid), block, 0, s>>>(a);
+    batch_attention_kernel<DP, true, W, RG><<<dim3(grid), dim3(64 * W), 0, s>>>(a);
   else
-    batch_attention_kernel<DP, false><<<dim3(grid), block, 0, s>>>(a);
+    batch_attention_kernel<DP, false, W, RG><<<dim3(grid), dim3(64 * W), 0, s>>>(a);
+}
+template <int DP, int W>
+void launch_w(const BatchArgs& a, int per_group, unsigned grid, hipStream_t s) {
+  if constexpr (DP <= 128)
+    if (per_group == 3) return launch_groups<DP, W, 3>(a, grid, s);
+  if constexpr (DP <= 192)
+    if (per_group == 2) return launch_groups<DP, W, 2>(a, grid, s);
+  launch_groups<DP, W, 1>(a, grid, s);
+}
+template <int DP>
+void launch(const BatchArgs& a, int per_group, unsigned grid, hipStream_t s) {
+  // Waves by what lies in LDS (16, 32, 64 KiB per wave at 64, 128, 256), two
+  // workgroups or more to a CU: one starts or ends while the other streams.  (16
+  // requests up to 4K, 32/8 heads of 128: 4 / 2 / 1 waves 45.7 / 39.1 / 42.6 us; 8
+  // up to 2K, 32/4 of 64: 11.5 / 13.0 / 13.9; 8 up to 4K, 16/8 of 256: 2 / 1 waves
+  // 45.8 / 38.9.)
+  launch_w<DP, (DP <= 64 ? 4 : DP <= 128 ? 2 : 1)>(a, per_group, grid, s);
 }
 
 bool batch_shape(int n_seqs, int nh, int nkv, int dph, int n_queries, int max_len, int bs) {
@@ -649,7 +741,7 @@ size_t sde_batch_attention_workspace_size(int n_seqs, int nh, int nkv, int dph, 
   using namespace sde::batch;
   if (!batch_shape(n_seqs, nh, nkv, dph, n_queries, max_len, block_size)) return 0;
   const int R = n_queries * (nh / nkv);
-  return batch_partial_bytes(batch_plan(n_seqs, nkv, R, max_len, block_size), n_seqs, nkv, R, dph);
+  return batch_partial_bytes(batch_plan(n_seqs, nkv, R, dph, max_len, block_size), n_seqs, nkv, R, dph);
 }
 
 int sde_batch_attention(const sde_batch_pool* pool, const int32_t* d_lens, int n_queries,
@@ -678,13 +770,14 @@ int sde_batch_attention(const sde_batch_pool* pool, const int32_t* d_lens, int n
 
   BatchArgs a;
   const int R = n_queries * (nh / nkv);
-  const BatchPlan p = batch_plan(pool->n_seqs, nkv, R, max_len, pool->block_size);
+  const BatchPlan p = batch_plan(pool->n_seqs, nkv, R, dph, max_len, pool->block_size);
   const size_t need = batch_partial_bytes(p, pool->n_seqs, nkv, R, dph);
   if (need > 0 && (!d_workspace || workspace_bytes < need ||
                    reinterpret_cast<uintptr_t>(d_workspace) % 16 != 0))
     return SDE_ERR_WORKSPACE;
   const int64_t grid = (int64_t)pool->n_seqs * nkv * p.row_groups * p.n_parts;
-  if (grid > (1 << 23)) return SDE_ERR_UNSUPPORTED;  // (a launch counts its threads in 32 bits)
+  // (a launch counts its threads in 32 bits)
+  if (grid > (1 << 23) || (int64_t)pool->n_seqs * nkv * R > (1 << 22)) return SDE_ERR_UNSUPPORTED;
   a.pool = pool->pool;
   a.tables = pool->tables;
   a.lens = d_lens;
@@ -717,24 +810,22 @@ int sde_batch_attention(const sde_batch_pool* pool, const int32_t* d_lens, int n
   const hipStream_t s = (hipStream_t)stream;
   const unsigned g = (unsigned)grid;
   if (dph <= 32)
-    launch<32>(a, g, s);
+    launch<32>(a, p.per_group, g, s);
   else if (dph <= 64)
-    launch<64>(a, g, s);
+    launch<64>(a, p.per_group, g, s);
   else if (dph <= 96)
-    launch<96>(a, g, s);
+    launch<96>(a, p.per_group, g, s);
   else if (dph <= 128)
-    launch<128>(a, g, s);
+    launch<128>(a, p.per_group, g, s);
   else if (dph <= 160)
-    launch<160>(a, g, s);
+    launch<160>(a, p.per_group, g, s);
   else if (dph <= 192)
-    launch<192>(a, g, s);
+    launch<192>(a, p.per_group, g, s);
   else
-    launch<256>(a, g, s);
+    launch<256>(a, p.per_group, g, s);
   const int ls = sde::launch_status();
   if (ls != SDE_OK || p.n_parts == 1) return ls;
-  const int64_t threads = (int64_t)pool->n_seqs * nkv * R * (dph / 4);
-  if ((threads + 255) / 256 > (1 << 23)) return SDE_ERR_UNSUPPORTED;
-  batch_combine_kernel<<<dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s>>>(a);
+  batch_combine_kernel<<<dim3((unsigned)(pool->n_seqs * nkv * R)), dim3(64 * kJoin), 0, s>>>(a);
   return sde::launch_status();
 }
 

@@ -8,10 +8,10 @@
 // the matrix cores and, beside them, one exponential, so:
 //  * a workgroup takes 128 rows -- (query, head in group) pairs of one KV head,
 //    so that the heads of a group share every key tile and short prompts still
-//    fill their tiles -- and its four waves 32 rows each;
-//  * tiles of 64 keys go from memory straight into LDS, one ahead of the one
-//    multiplied (two buffers, one barrier a tile), K and V rows swizzled so that
-//    operand reads use all banks;
+//    fill their tiles -- or 256 of long prompts, and each of its waves 32;
+//  * tiles of 64 keys go from memory straight into LDS, one or three ahead of the
+//    one multiplied (one barrier a tile), K and V rows swizzled so that operand
+//    reads use all banks;
 //  * S^T = K q^T by 32x32x16 MFMA leaves a lane with one row's logits; in that
 //    order they are its operand of O^T = V^T P^T, so the softmax exchanges
 //    nothing but the row's max and sum, between two lanes;
@@ -21,6 +21,12 @@
 //    is raised only when a logit is 2^8 above it.
 //  * row tiles start from the end of the packed rows, where they are longest;
 //    the KV head is the fastest index: with 8 of them each XCD's L2 holds one's.
+//
+// Measured on MI355X: one prompt of 8192 tokens, 32/8 heads of 128: 534 us in fp16,
+// 1029 TFLOP/s, 504 us in bf16, 1091 (a square product of 8192 reaches 1184 and
+// 1238 in the library); of 4096 147 us, 934 TFLOP/s; six uneven prompts of 4093
+// tokens in all 46-54 us: some 3000 cycles pass from a tile's logits to its output
+// in one wave, and short prompts have too few waves to hide them.
 #include <cmath>
 
 #include "batch_common.hpp"
@@ -39,9 +45,6 @@ typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kRows = 32 * kWaves;  // rows of a workgroup
 constexpr int kTok = 64;            // keys per tile
 constexpr int kBatch = 2;             // k-steps whose operands are read together
 constexpr float kLazyMax = 8.f;
@@ -53,26 +56,34 @@ struct PromptArgs {
   uint16_t* out;
   const int32_t* starts;
   int64_t q_stride, k_stride, v_stride, out_stride;
-  int n_tokens, n_seqs, nkv, G, dph, tiles;
+  int n_tokens, n_seqs, nkv, G, dph;
+  int rows, tiles;  // rows of a workgroup, row tiles
   float scale;  // log2(e) / sqrt(dph)
 };
 
-template <int DP>
+// WAVES of 32 rows.  Eight: one workgroup to a CU, four tiles of keys in LDS, three
+// on their way.  Four: two workgroups to a CU (head sizes up to 128), two tiles
+// each.
+template <int DP, int WAVES>
 struct Shape {
+  static constexpr int THREADS = 64 * WAVES;
+  static constexpr int ROWS = 32 * WAVES;
+  static constexpr int STAGES = WAVES == 8 ? 4 : 2;
   static constexpr int UNITS = DP / 8;      // 16-byte units per staged row
   static constexpr int KS = DP / 16;        // k-steps of the logits product
   static constexpr int DB = DP / 32;        // 32-feature blocks of the output
   static constexpr int ROWB = 2 * DP;
   static constexpr int TILEB = kTok * ROWB;
-  static constexpr int NU = TILEB / (16 * kThreads);  // loads per thread, K or V
+  static_assert(TILEB % (16 * THREADS) == 0, "a tile is whole loads of every thread");
+  static constexpr int NU = TILEB / (16 * THREADS);  // loads per thread, K or V
 };
 
 // Place of unit u of token t's row: u ^ swizzle(t).  Any 16 tokens read at one
 // unit, and 8 tokens read over 64 bytes, use all 64 banks evenly.
 template <int DP>
 __device__ __forceinline__ int swizzle(int t) {
-  if constexpr (Shape<DP>::UNITS % 16 == 0) return ((t & 3) << 2) | ((t >> 2) & 3);
-  if constexpr (Shape<DP>::UNITS % 8 == 0) return (((t >> 1) & 1) << 2) | ((t >> 2) & 3);
+  if constexpr (DP % 128 == 0) return ((t & 3) << 2) | ((t >> 2) & 3);
+  if constexpr (DP % 64 == 0) return (((t >> 1) & 1) << 2) | ((t >> 2) & 3);
   return (t >> 2) & 3;
 }
 
@@ -87,7 +98,11 @@ __device__ __forceinline__ void load_to_lds(const uint16_t* p, uint32_t off, uin
       : "s"(lds_off), "v"(off), "s"(p)
       : "memory");
 }
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "vmcnt counts to 63");
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
 
 template <bool BF16>
 __device__ __forceinline__ f16v mfma(u4v a, u4v b, f16v c) {
@@ -125,11 +140,11 @@ __device__ __forceinline__ float half_max(float x) {
 }
 
 // Row tiles are numbered so that sequence b's begin at
-// first_tile(b) = starts[b] * G / kRows + b: at least as many numbers as it has
+// first_tile(b) = starts[b] * G / rows + b: at least as many numbers as it has
 // tiles, without a sum over the sequences before it.
 __device__ __forceinline__ int64_t first_tile(const PromptArgs& a, int b) {
   const int s = min(max(a.starts[b], 0), a.n_tokens);
-  return (int64_t)s * a.G / kRows + b;
+  return (int64_t)s * a.G / a.rows + b;
 }
 
 // The last sequence whose tiles begin at or before t (starts[0]'s at worst).
@@ -149,10 +164,11 @@ __device__ __forceinline__ int sequence_of(const PromptArgs& a, int64_t t) {
   return wave_uniform(lo);
 }
 
-template <int DP, bool FULL, bool BF16>
-__global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void prompt_kernel(PromptArgs a) {
-  using Sh = Shape<DP>;
-  __shared__ __attribute__((aligned(1024))) char lds[2][2 * Sh::TILEB];  // [buffer][K, V]
+template <int DP, bool FULL, bool BF16, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 || DP <= 128 ? 2 : 1) void prompt_kernel(PromptArgs a) {
+  using Sh = Shape<DP, WAVES>;
+  constexpr int kThreads = Sh::THREADS, kRows = Sh::ROWS, S = Sh::STAGES;
+  __shared__ __attribute__((aligned(1024))) char lds[S][2 * Sh::TILEB];  // [buffer][K, V]
   __shared__ int first_bad[DP], any_bad;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -194,13 +210,13 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void prompt_kernel(Prom
   if (!FULL) {
     // the features beyond the head's, which no load reaches
     const uint4 z = make_uint4(0, 0, 0, 0);
-    for (int i = tid; i < 2 * 2 * Sh::TILEB / 16; i += kThreads)
+    for (int i = tid; i < S * 2 * Sh::TILEB / 16; i += kThreads)
       reinterpret_cast<uint4*>(&lds[0][0])[i] = z;
     __syncthreads();
   }
   const uint32_t k_row = 2u * (uint32_t)a.k_stride, v_row = 2u * (uint32_t)a.v_stride;
   auto load_tile = [&](int kt) {
-    const uint32_t dst = lds0 + (uint32_t)(kt & 1) * (2 * Sh::TILEB);
+    const uint32_t dst = lds0 + (uint32_t)(kt % S) * (2 * Sh::TILEB);
     const uint16_t* const kp = kb + (int64_t)kt * kTok * a.k_stride;
     const uint16_t* const vp = vb + (int64_t)kt * kTok * a.v_stride;
     const int left = n - 1 - kt * kTok;  // (the clamp's only use: a sequence's end)
@@ -216,7 +232,9 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void prompt_kernel(Prom
       }
     }
   };
-  load_tile(0);
+#pragma unroll
+  for (int i = 0; i < S - 1; i++)
+    if (i < tiles) load_tile(i);
   for (int i = tid; i < DP; i += kThreads) first_bad[i] = INT32_MAX;
   if (tid == 0) any_bad = 0;
   __syncthreads();
@@ -231,6 +249,10 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void prompt_kernel(Prom
       qf[ks] = u4v{0, 0, 0, 0};
       if (FULL || f < a.dph) qf[ks] = *reinterpret_cast<const u4v*>(qp + f);
     }
+    // (waited for here: left to their first use, in the loop, the waits would
+    // count the next tile's loads too, which the compiler does not know)
+#pragma unroll
+    for (int ks = 0; ks < Sh::KS; ks++) asm volatile("" : "+v"(qf[ks]));
   }
 
   float ref = 0.f, raise = -INFINITY, l = 0.f;
@@ -249,13 +271,23 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void prompt_kernel(Prom
   int kx = 16 * (hf ^ swizzle<DP>(l32)), vx = 16 * (vu ^ swizzle<DP>(vt));
 
   for (int kt = 0; kt < tiles; kt++) {
-    char* const kst = &lds[kt & 1][0];
+    char* const kst = &lds[kt % S][0];
     char* const vst = kst + Sh::TILEB;
     const int ts = kt * kTok;
     // (opaque here: kept across the loop, the addresses of all reads take more
     // registers than there are)
     asm volatile("" : "+v"(kx), "+v"(vx));
-    wait_loads();
+    // tile kt is here; those behind it may be on their way
+    if constexpr (S == 4) {
+      if (kt + 2 < tiles)
+        wait_loads<4 * Sh::NU>();
+      else if (kt + 1 < tiles)
+        wait_loads<2 * Sh::NU>();
+      else
+        wait_loads<0>();
+    } else {
+      wait_loads<0>();
+    }
     if (ts + kTok - 1 > q0) {
       // Keys that some row of the workgroup does not see: a V element there
       // that is not finite must not meet a weight of 0.  It becomes 0, and the
@@ -280,7 +312,8 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void prompt_kernel(Prom
       }
     }
     __syncthreads();
-    if (kt + 1 < tiles) load_tile(kt + 1);
+    // (every wave is past tile kt - 1, whose buffer this is)
+    if (kt + S - 1 < tiles) load_tile(kt + S - 1);
     if (ts > w_last) continue;  // (wave-uniform)
 
     f16v s[2];
@@ -402,30 +435,40 @@ __global__ __launch_bounds__(kThreads, DP > 128 ? 1 : 2) void prompt_kernel(Prom
     }
 }
 
-template <int DP, bool BF16>
-void launch(const PromptArgs& a, unsigned grid, hipStream_t s) {
+template <int DP, bool BF16, int WAVES>
+void launch_waves(const PromptArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(a.tiles * a.nkv)), block(64 * WAVES);
   if (a.dph == DP)
-    prompt_kernel<DP, true, BF16><<<dim3(grid), dim3(kThreads), 0, s>>>(a);
+    prompt_kernel<DP, true, BF16, WAVES><<<grid, block, 0, s>>>(a);
   else
-    prompt_kernel<DP, false, BF16><<<dim3(grid), dim3(kThreads), 0, s>>>(a);
+    prompt_kernel<DP, false, BF16, WAVES><<<grid, block, 0, s>>>(a);
+}
+
+template <int DP, bool BF16>
+void launch(const PromptArgs& a, hipStream_t s) {
+  if (a.rows == 256) {
+    if constexpr (DP % 64 == 0 && DP <= 128) launch_waves<DP, BF16, 8>(a, s);
+  } else {
+    launch_waves<DP, BF16, 4>(a, s);
+  }
 }
 
 template <bool BF16>
-void launch_type(const PromptArgs& a, unsigned grid, hipStream_t s) {
+void launch_type(const PromptArgs& a, hipStream_t s) {
   if (a.dph <= 32)
-    launch<32, BF16>(a, grid, s);
+    launch<32, BF16>(a, s);
   else if (a.dph <= 64)
-    launch<64, BF16>(a, grid, s);
+    launch<64, BF16>(a, s);
   else if (a.dph <= 96)
-    launch<96, BF16>(a, grid, s);
+    launch<96, BF16>(a, s);
   else if (a.dph <= 128)
-    launch<128, BF16>(a, grid, s);
+    launch<128, BF16>(a, s);
   else if (a.dph <= 160)
-    launch<160, BF16>(a, grid, s);
+    launch<160, BF16>(a, s);
   else if (a.dph <= 192)
-    launch<192, BF16>(a, grid, s);
+    launch<192, BF16>(a, s);
   else
-    launch<256, BF16>(a, grid, s);
+    launch<256, BF16>(a, s);
 }
 
 }  // namespace prompt
@@ -468,14 +511,21 @@ extern "C" int sde_prompt_attention(const int32_t* d_starts, int n_seqs, int n_t
   a.nkv = nkv;
   a.G = nh / nkv;
   a.dph = dph;
-  const int64_t tiles = (int64_t)n_tokens * a.G / kRows + n_seqs;
-  if (tiles * nkv > (1 << 23)) return SDE_ERR_UNSUPPORTED;  // (threads of a launch: 32 bits)
+  // 256 rows of long prompts: each key tile is brought in once for twice the
+  // rows, if that still makes two workgroups per CU.  Measured on MI355X, 128 / 256
+  // rows, us: one prompt of 8192 tokens, 32/8 heads of 128, fp16 629 / 534, bf16 598
+  // / 504, of 4096 184 / 147; four of 1024 72 / 68, six of 680 on average, uneven,
+  // 54 / 62; 8/8 heads, 4096 tokens (128 workgroups) 89 / 106; 32/4 heads of 64,
+  // 4096 99.7 / 99.3.
+  const bool whole = (dph > 32 && dph <= 64) || (dph > 96 && dph <= 128);  // (Shape's NU)
+  a.rows = whole && (int64_t)n_tokens * nh >= 512 * 256 && n_tokens / n_seqs >= 1024 ? 256 : 128;
+  const int64_t tiles = (int64_t)n_tokens * a.G / a.rows + n_seqs;
+  if (tiles * nkv > (1 << 22)) return SDE_ERR_UNSUPPORTED;  // (threads of a launch: 32 bits)
   a.tiles = (int)tiles;
   a.scale = (float)(1.4426950408889634 / std::sqrt((double)dph));
-  const unsigned grid = (unsigned)(tiles * nkv);
   if (dtype == SDE_F16)
-    launch_type<false>(a, grid, (hipStream_t)stream);
+    launch_type<false>(a, (hipStream_t)stream);
   else
-    launch_type<true>(a, grid, (hipStream_t)stream);
+    launch_type<true>(a, (hipStream_t)stream);
   return sde::launch_status();
 }

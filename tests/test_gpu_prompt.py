@@ -94,6 +94,37 @@ def test_lengths(gpu, lens):
     check(out, want, mag, F16)
 
 
+@pytest.mark.parametrize("nh,nkv,dph,lens,dtype", [
+    (64, 8, 64, [1030, 1070], F16), (64, 2, 56, [2100], BF16), (32, 8, 128, [2101, 2099], BF16),
+    (32, 8, 128, [4111], F16), (32, 32, 120, [1, 4201, 0], F16)])
+def test_long_prompts(gpu, nh, nkv, dph, lens, dtype):
+    """Enough rows of long prompts for workgroups of 256."""
+    rng = np.random.default_rng(nh + dph)
+    starts, tail = ends(lens), 3
+    g = torch.Generator(device="cuda").manual_seed(nh + dph)
+    T = starts[-1] + tail
+    q, k, v = (torch.randn(T, w, generator=g, device="cuda").to(dtype)
+               for w in (nh * dph, nkv * dph, nkv * dph))
+    out = torch.full((T, nh * dph), 0.5, dtype=dtype, device="cuda")
+    case_banner("prompt_attention long", nh, nkv, dph, lens, dtype)
+    st = torch.tensor(starts, dtype=torch.int32).cuda()
+    prompt_attention(q, k, v, st, nh, nkv, dph, out=out)
+    want, mag = reference(q, k, v, starts, nh, nkv, dph)
+    check(out[:-tail], want[:-tail], mag[:-tail], dtype)
+    assert (out[-tail:] == 0.5).all()
+    # a key and a value that are not finite, at the longest one's middle
+    b = int(np.argmax(lens))
+    at = starts[b] + lens[b] // 2 + int(rng.integers(0, 64))
+    k[at, :dph] = float("nan")
+    v[at, -1] = float("inf")
+    prompt_attention(q, k, v, st, nh, nkv, dph, out=out)
+    rest = [i for i in range(starts[-1]) if not at <= i < starts[b + 1]]
+    check(out[rest], want[rest], mag[rest], dtype)
+    later = out[at:starts[b + 1]].float().view(-1, nh, dph)
+    assert torch.isnan(later[:, :nh // nkv]).all()
+    assert not torch.isfinite(later[:, nh - nh // nkv:, -1]).any()
+
+
 def test_starts_out_of_order_or_range(gpu):
     """Rows before the first start stay; starts beyond the rows count as their
     end; a falling start leaves its rows out; nothing else is touched."""

@@ -708,7 +708,7 @@ __device__ __forceinline__ Kept last_kept(const RowView<E>& row, const Weight& w
 // One workgroup walks a row of 128256 at some 20 us a time where weights are
 // needed.  With fewer rows than fill the chip, a row is cut into slices of
 // vectors, a workgroup each, in three launches before the row's own:
-//  max      the slice's max;
+//  max      the slice's max, and for top-k each thread's;
 //  weights  top-k above kList, or top-p: the slice's histogram, of tokens or of
 //           weight, and its total; the last workgroup of a row joins them and
 //           finds the bin that holds the last kept token;
@@ -717,9 +717,8 @@ __device__ __forceinline__ Kept last_kept(const RowView<E>& row, const Weight& w
 //           before it.
 // The row's workgroup then has the lists to compare, and the slices' weights
 // to find the one that holds the token, which alone it walks.
-// Which way a row goes is told by its parameters.  Rows with k up to kList leave
-// the slices alone (two light walks: 128256 fp32 values 24 us in one workgroup,
-// 34 with a cut and lists from 16 slices), and one whose list would be too long (flat rows, ties), or with
+// Which way a row goes is told by its parameters.  Rows with k up to kList take
+// the threads' maxima and one light walk by their own workgroup; one whose list would be too long (flat rows, ties), or with
 // both a large k and top-p, is walked whole by its workgroup.
 
 enum class Way { kTop, kTopK, kRank, kNucleus, kTotals, kWhole };
@@ -768,6 +767,7 @@ struct SliceArgs {
   int S;                      // slices of a row
   float* top;                 // [rows][S]
   int* first;                 // [rows][S]
+  float* thread_top;          // [rows][S][kSliceThreads], where top-k acts
   double* total;              // [rows][S]; after the gather: the weight before bin lo
   unsigned long long* mass;   // [rows][S][kSliceBins] (tokens, where top-k acts)
   uint32_t* listed;           // [rows][S]
@@ -845,7 +845,6 @@ template <class E>
 __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SliceArgs sa) {
   __shared__ SliceLds s;
   const int r = blockIdx.y, sl = blockIdx.x, tid = threadIdx.x;
-  if (RowParams(sa.a, r).way == Way::kTopK) return;
   const SliceView<E> view(sa, r, sl);
   float x = -INFINITY;
   int i = -1;
@@ -856,6 +855,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SliceArgs sa)
     }
   });
   const size_t rs = (size_t)r * sa.S + sl;
+  if (RowParams(sa.a, r).way == Way::kTopK) sa.thread_top[rs * kSliceThreads + tid] = x;
   wave_top(x, i);
   if ((tid & 63) == 0) {
     s.wave_f[tid >> 6] = x;
@@ -875,16 +875,19 @@ __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SliceArgs sa)
   }
 }
 
-// The lowest key (of a finite value) in bins up to b; the max's is in bin 0.
+// The lowest key (of a finite value) in bins up to b; the max's is in bin 0.  A
+// whole wave calls it: 63 places of the range at a time.
 __device__ __forceinline__ uint32_t lowest_key(const Weight& weight, int b) {
+  const uint32_t lane = threadIdx.x & 63;
   uint32_t lo = key_of(-FLT_MAX), hi = key_of(weight.top);
 #pragma unroll 1
   while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    if (weight.bin(value_of_key(mid)) <= b)
-      hi = mid;
-    else
-      lo = mid + 1;
+    const uint32_t step = (hi - lo) / 63 + 1;
+    const uint32_t at = lane * step < hi - lo ? lo + lane * step : hi;  // (hi is one)
+    const uint64_t in = __builtin_amdgcn_ballot_w64(weight.bin(value_of_key(at)) <= b);
+    const int first = __builtin_ctzll(in);
+    hi = __builtin_amdgcn_readlane(at, first);
+    if (first > 0) lo = __builtin_amdgcn_readlane(at, first - 1) + 1;
   }
   return lo;
 }
@@ -1012,10 +1015,14 @@ __global__ __launch_bounds__(kSliceThreads) void sample_weights_kernel(SliceArgs
   }
   // The values in those bins (bins rise as values fall), by bisection: two
   // compares tell in what follows.
-  if (tid == 0) sa.info[r].low = value_of_key(lowest_key(weight, min(hi, kSliceBins - 1)));
-  if (tid == 64)
-    sa.info[r].high =
+  if (tid < 64) {
+    const float low = value_of_key(lowest_key(weight, min(hi, kSliceBins - 1)));
+    if (tid == 0) sa.info[r].low = low;
+  } else if (tid < 128) {
+    const float high =
         lo == 0 ? INFINITY : value_of_key(lowest_key(weight, min(lo, kSliceBins) - 1) - 1);
+    if (tid == 64) sa.info[r].high = high;
+  }
 }
 
 template <class E>
@@ -1147,14 +1154,22 @@ __device__ __forceinline__ void finish_few(const SampleArgs& a, int r, const Row
   }
 }
 
-// The lowest of the threads' maxima that at least k of them reach (to 8 bins).
-__device__ __forceinline__ float top_k_low(Lds& s, const Weight& weight, float mine, int k) {
+// The lowest of the given maxima of parts of the row, kTops per thread, that at
+// least k of them reach (to 8 bins): at least k tokens do.
+constexpr int kTops = kMaxSlices * kSliceThreads / kThreads;
+
+__device__ __forceinline__ float top_k_low(Lds& s, const Weight& weight, const float (&x)[kTops],
+                                           int k) {
   constexpr int N = kBins / 8;
   const int tid = threadIdx.x;
   if (tid < N) s.count[tid] = 0;
   __syncthreads();
-  const int b = weight.bin(mine);
-  if (b < kBins) atomicAdd(&s.count[b / 8], 1u);
+  int b[kTops];
+#pragma unroll
+  for (int i = 0; i < kTops; i++) {
+    b[i] = weight.bin(x[i]);
+    if (b[i] < kBins) atomicAdd(&s.count[b[i] / 8], 1u);
+  }
   __syncthreads();
   if (tid < 64) {
     const uint4 c = *reinterpret_cast<const uint4*>(&s.count[4 * tid]);
@@ -1181,7 +1196,11 @@ __device__ __forceinline__ float top_k_low(Lds& s, const Weight& weight, float m
   __syncthreads();
   const int cut = s.found;
   if (cut == kBins) return -FLT_MAX;  // fewer hold a token of weight: every one
-  if (b <= cut) atomicMin(&s.lo, key_of(mine));
+  uint32_t low = 0xFFFFFFFFu;
+#pragma unroll
+  for (int i = 0; i < kTops; i++)
+    if (b[i] <= cut) low = min(low, key_of(x[i]));
+  if (low != 0xFFFFFFFFu) atomicMin(&s.lo, low);
   __syncthreads();
   return value_of_key(s.lo);
 }
@@ -1200,12 +1219,23 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
 
   fill_powers<kThreads>(s.power);
   // ---- the max, and its first index
-  float mine = -INFINITY;
+  float part_top[kTops];  // maxima of parts of the row, for top-k
+#pragma unroll
+  for (int i = 0; i < kTops; i++) part_top[i] = -INFINITY;
   float top;
   int first;
-  if (SLICED && q.way != Way::kTopK) {
+  if constexpr (SLICED) {
+    if (q.way == Way::kTopK) {
+      const float* t = sa.thread_top + (size_t)r * sa.S * kSliceThreads;
+#pragma unroll
+      for (int i = 0; i < kTops; i++) {
+        const int j = i * kThreads + threadIdx.x;
+        if (j < sa.S * kSliceThreads) part_top[i] = t[j];
+      }
+    }
     row_top(sa, r, top, first);
   } else {
+    float mine = -INFINITY;
     int at = -1;
     row.template walk<true>(w0, w1, [&](float v, int i) {
       if (v > mine) {
@@ -1213,6 +1243,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
         at = i;
       }
     });
+    part_top[0] = mine;
     float x = mine;
     wave_top(x, at);
     if (lane == 0) {
@@ -1249,7 +1280,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
   bool ready = false;     // the whole row's histogram is there
   bool slices = false;    // the row's weight is in its slices, the list only its last part
   if (q.way == Way::kTopK) {
-    const float low = top_k_low(s, weight, mine, q.k);
+    const float low = top_k_low(s, weight, part_top, q.k);
     n = collect<true>(row, s, [&](float v, int) { return v >= low; });
   } else if constexpr (SLICED) {
     if (q.way == Way::kNucleus || q.way == Way::kRank) {
@@ -1400,14 +1431,15 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SliceArgs sa) {
 
 struct Layout {
   int S = 1;  // 1: no slices
-  size_t first = 0, total = 0, mass = 0, listed = 0, list = 0, info = 0,
+  size_t first = 0, thread_top = 0, total = 0, mass = 0, listed = 0, list = 0, info = 0,
          arrived = 0, bytes = 0;
 };
 
 // Some 1024 slices over all rows, 16 of a row at most, from 32768 tokens on:
-// below, four launches cost what they save (one row of 32000, no filter 22 us
-// whole / 25 in slices, k = 50 17 / 25; of 128256 55 / 28, 24 / 28, p = 0.9 222 /
-// 50; 192 rows of 128256 68 / 75, 42 / 48, 246 / 120).
+// below, four launches cost what they save.  Measured on MI355X, us whole / in
+// slices, fp32: one row of 32000, no filter 22 / 25, k = 50 16 / 25, p = 0.9 51 / 43;
+// of 128256 55 / 27, 24 / 26, 222 / 44; 192 rows of 128256 68 / 74, 42 / 51, 246 /
+// 122.
 Layout layout_of(int rows, int V) {
   Layout l;
   int64_t S = (1024 + (int64_t)rows - 1) / rows;
@@ -1423,6 +1455,7 @@ Layout layout_of(int rows, int V) {
   };
   put(n * 4);  // top
   l.first = put(n * 4);
+  l.thread_top = put(n * 4 * kSliceThreads);
   l.total = put(n * 8);
   l.mass = put(n * 8 * kSliceBins);
   l.listed = put(n * 4);
@@ -1488,6 +1521,7 @@ int sde_sample(const void* d_logits, int64_t row_stride, int dtype, int n_rows, 
     char* w = static_cast<char*>(d_workspace);
     sa.top = reinterpret_cast<float*>(w);
     sa.first = reinterpret_cast<int*>(w + l.first);
+    sa.thread_top = reinterpret_cast<float*>(w + l.thread_top);
     sa.total = reinterpret_cast<double*>(w + l.total);
     sa.mass = reinterpret_cast<unsigned long long*>(w + l.mass);
     sa.listed = reinterpret_cast<uint32_t*>(w + l.listed);

@@ -28,9 +28,10 @@
 //  * the max is raised only when a logit is 2^8 above it.
 //
 // Measured on MI355X (graph replays over three inputs), 32/8 heads of 128 where
-// not said: 96 requests up to 8K, bf16, 1.64 GB: 323 us, 5.1 TB/s (a copy of 4 GiB
-// runs at 4.7); 16 up to 4K, 149 MB: 39 us, 3.8 TB/s; one of 32K: 35 us, 3.9; the
-// 5-query verify of 3 up to 32K, 28/4 heads, 144 MB: 55 us, the combine's 8 in it.
+// not said: 96 requests up to 8K, bf16, 1.64 GB: 318 us, 5.2 TB/s (a copy of 4 GiB
+// runs at 4.7); 16 up to 4K, 149 MB: 38 us, 3.9 TB/s; one of 32K: 35 us, 3.9; the
+// 5-query verify of 3 up to 32K, 28/4 heads, 144 MB: 47 us, 3.1 TB/s, the combine's
+// 5 in it.
 // Short of the bandwidth there: some 4 us pass before a workgroup's first tile is
 // there (length and table, then K), and partitions end unevenly.
 #include <algorithm>
@@ -579,9 +580,10 @@ __global__ __launch_bounds__(64 * W) void batch_attention_kernel(BatchArgs a) {
 }
 
 // Joins a row's partitions: a workgroup per row, kJoin of its threads side by
-// side over a 16-byte unit's partitions, whose sums meet in LDS in order.
-constexpr int kJoin = 8;
-
+// side over a 16-byte unit's partitions, whose sums meet in LDS in order.  Eight
+// for more than eight partitions (43 each of 420 rows: 15.6 us by one, 5.2 by
+// eight; 5 each of 96 x 32 rows: 5.7 and 9.1).
+template <int kJoin>
 __global__ __launch_bounds__(64 * kJoin) void batch_combine_kernel(BatchArgs a) {
   __shared__ float4 part_y[kJoin][64];
   __shared__ float2 part_ml[kJoin];
@@ -675,10 +677,11 @@ int groups_per(int R, int dph) {
 // evens out the requests' lengths: up to 4096 workgroups, over 512 positions or
 // more, from two units per CU on over 1024.  Measured on MI355X, us per call by
 // the number of workgroups aimed at (512 / 768 / 4096), 32/8 heads of 128: 16
-// requests up to 4K 41.1 / 39.1 / 45, one of 32K 35.6 / 36 / 45, the 5-query verify
-// of 3 up to 32K 55 / 66 / 90, 40 up to 2K 61.9 / 61 / 56.5, 96 up to 8K 367 / 367 /
-// 323; 128 up to 1K with 1024 positions at least 67, with 256 98.  No partition
-// has more table entries than fit LDS.
+// requests up to 4K 41.1 / 39.1 / 45 (640: 38.4), one of 32K 35.6 / 36 / 45, the
+// 5-query verify of 3 up to 32K 55 / 66 / 90 (640, with a faster combine: 47), 40 up
+// to 2K 61.9 / 61 / 56.5, 96 up to 8K 367 / 367 / 323 (318 with the faster combine);
+// 128 up to 1K with 1024 positions at least 67, with 256 98.  No partition has more
+// table entries than fit LDS.
 BatchPlan batch_plan(int n_seqs, int nkv, int R, int dph, int max_len, int bs) {
   BatchPlan p;
   p.per_group = groups_per(R, dph);
@@ -825,7 +828,11 @@ int sde_batch_attention(const sde_batch_pool* pool, const int32_t* d_lens, int n
     launch<256>(a, p.per_group, g, s);
   const int ls = sde::launch_status();
   if (ls != SDE_OK || p.n_parts == 1) return ls;
-  batch_combine_kernel<<<dim3((unsigned)(pool->n_seqs * nkv * R)), dim3(64 * kJoin), 0, s>>>(a);
+  const dim3 joins((unsigned)(pool->n_seqs * nkv * R));
+  if (p.n_parts > 8)
+    batch_combine_kernel<8><<<joins, dim3(512), 0, s>>>(a);
+  else
+    batch_combine_kernel<1><<<joins, dim3(64), 0, s>>>(a);
   return sde::launch_status();
 }
 

@@ -24,11 +24,19 @@
 // last token down by further histograms over ranges of x, then walk the row
 // once more for the total in index order and a 16th of it for the token.
 //
-// Weights and sums are 64-bit (an fp64 multiply-add issues at the rate of an
-// fp32 one): which token is drawn hangs on a sum's side of u * total, and fp32
-// sums over 128256 tokens would take the neighbour in some 2 % of rows.  The
-// histogram's weights are 64-bit fixed-point sums: atomics in any order give
-// the same bits.
+// Weights and sums are 64-bit: which token is drawn hangs on a sum's side of
+// u * total, and fp32 sums over 128256 tokens would take the neighbour in some
+// 2 % of rows.  The histogram's weights are 64-bit fixed-point sums: atomics in
+// any order give the same bits.
+//
+// Long rows that do not fill the chip by themselves go in slices: maxima, weights
+// and lists are made by kernels with a workgroup per slice, and the row's own
+// workgroup starts at step 3.
+//
+// Measured on MI355X: one fp32 row of 32000 15.4 us, a chain of walks by one
+// workgroup; 24 fp32 rows of 128256 under top-k and top-p 58 us (max 5.7, weights 21,
+// list 8.7, row 23); 192 bf16 ones 117 us (12, 55, 15, 35 to 42): the 64-bit
+// weights and their histogram, not the 49 MB, take the time.
 #include <cfloat>
 #include <cmath>
 
@@ -206,7 +214,7 @@ struct RowView {
   // (NaN passes no compare and weighs nothing)
   static __device__ __forceinline__ float value(T e) { return E::get(e); }
   // f(value, index) over a vector's elements, in pairs: the loop is rolled, since
-  // an exponential's code a dozen times over costs more to fetch than to run.
+  // f unrolled eight times over spilled registers (the time is the same).
   template <class F>
   static __device__ __forceinline__ void each(uint4 c, int index, F f) {
 #pragma unroll 1

@@ -102,6 +102,27 @@ def test_attention_partitions(gpu, nh, nkv, dph, bs, lens, m):
     check(got, attention_f64(q, pool, tables, lens, nh, nkv, dph, m), F32, 1e-4)
 
 
+@pytest.mark.parametrize("nh,nkv,dph,bs,lens,m,parts", [
+    (8, 4, 72, 16, [1500, 0, 513, 512] + [40] * 66, 1, 3), (8, 4, 256, 16, [2000, 1, 0, 257, 1999], 1, 8),
+    (8, 4, 80, 16, [2300, 256, 0, 2], 2, 9), (28, 4, 128, 16, [9000, 3, 4700, 5], 5, 36),
+    (8, 2, 64, 16, [20000, 6], 1, 79)])
+def test_attention_joins(gpu, nh, nkv, dph, bs, lens, m, parts):
+    """Few and many partitions of a row, of which a short request fills one or none.
+    Joining adds a rounding of fp32 per partition, far below the tolerance of a
+    row of one."""
+    rng = np.random.default_rng(17)
+    case_banner("batch_attention joins", nh, nkv, dph, bs, m, parts)
+    size = batch_attention_workspace_size(len(lens), nh, nkv, dph, m, max(lens), bs)
+    assert size == len(lens) * nh * m * parts * (dph + 2) * 4
+    pool, tables = make_pool(rng, lens, bs, nkv * dph)
+    q = torch.from_numpy(rng.standard_normal((len(lens) * m, nh * dph))).float().cuda()
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    got = batch_attention(q, pool, tables, n, nh, nkv, dph, n_queries=m, max_len=max(lens))
+    check(got, attention_f64(q, pool, tables, lens, nh, nkv, dph, m), F32, 1e-4)
+    again = batch_attention(q, pool, tables, n, nh, nkv, dph, n_queries=m, max_len=max(lens))
+    assert torch.equal(got, again)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_nonfinite_where_hidden(gpu, dtype):
     """NaN and infinities of a window's later tokens do not reach the earlier

@@ -22,12 +22,13 @@
 //  * row tiles start from the end of the packed rows, where they are longest;
 //    the KV head is the fastest index: with 8 of them each XCD's L2 holds one's.
 //
-// Measured on MI355X: one prompt of 8192 tokens, 32/8 heads of 128: 526 to 556 us in
-// fp16 by the card, 988 to 1045 TFLOP/s, 504 us in bf16, 1091 (a square product of 8192 reaches 1184 and
-// 1238 in the library), the matrix cores busy for half of the SIMDs' cycles and the
-// vector unit for 44 %, no bank conflicts; of 4096 147 us, 934 TFLOP/s; six uneven
-// prompts of 4093 tokens in all 47 us, 580 TFLOP/s: some 3000 cycles pass from a tile's logits to its output
-// in one wave, and short prompts have too few waves to hide them.
+// Measured on MI355X: one prompt of 8192 tokens, 32/8 heads of 128: 526 to 556 us
+// in fp16 by the card, 988 to 1045 TFLOP/s, 504 us in bf16, 1091 (a square product
+// of 8192 reaches 1184 and 1238 in the library), the matrix cores busy for half of
+// the SIMDs' cycles and the vector unit for 44 %, no bank conflicts; of 4096 147
+// us, 934 TFLOP/s; six uneven prompts of 4093 tokens in all 47 us, 580 TFLOP/s:
+// some 3000 cycles pass from a tile's logits to its output in one wave, and short
+// prompts have too few waves to hide them.
 #include <cmath>
 
 #include "batch_common.hpp"
